@@ -11,9 +11,13 @@
 // histograms over ever smaller ranges of values, plus the number m of values equal to K that are still
 // kept (the first m by index).
 //
-// Weights are integers: exp in 64 bits, scaled by 2^S (2^44) and rounded.  Their sums are exact, so neither the
-// split over threads and CTAs nor the order of the atomics changes a result, and a decision next to a
-// border is the one that 64-bit arithmetic makes (a weight is off by 2^-42 of itself or 2^-45 of the largest).
+// Weights are integers: exp in 64 bits, scaled by 2^84 and rounded, in two words that are added up apart (2^43, and a
+// signed rest).  Their sums are exact, so neither the split over threads and CTAs nor the order of the atomics changes a
+// result, and a decision next to a border is the one that 64-bit arithmetic makes, in a long tail of tiny weights too:
+// a weight is off by 2^-42 of itself and 2^-85 of the largest.  With one word of 2^44 a tail at 2^-45 of the largest was
+// lost altogether, 2^-28 of the whole at V = 128256.  The histogram of top-p takes them in steps of 2^-43, and where a
+// border is not clear by what that may be off (few rows) again in steps of 2^-59, so top-p is right to V 2^-60 of the
+// whole.  What rounds to zero even so is only ever chosen at u = 0.
 //
 // A thread-block cluster owns a row: each CTA stages its slice of the row in shared memory (read once
 // from HBM) and the passes run there; histograms, maxima and sums meet through distributed shared memory.
@@ -29,10 +33,13 @@
 #include "common.cuh"
 #include "capi_internal.h"
 #include <math.h>
+#include <stddef.h>
+#include <type_traits>
 
 namespace arke {
 
 typedef unsigned long long u64;
+typedef unsigned __int128 u128;
 
 constexpr int kSmpThreads = 512;
 constexpr int kSmpWarps = kSmpThreads / 32;
@@ -52,7 +59,6 @@ struct SampleParams {
   int64_t* token;
   float* logprob;
   int B, V, slice, staged, stage_at;
-  int scale;           // S: 44, or as much as lets V weights of 2^S add up in 64 bits
 };
 
 template <typename T> struct SmpType;
@@ -113,18 +119,62 @@ __device__ __forceinline__ u64 warp_scan(u64 v) {   // inclusive
   return v;
 }
 
+__device__ __forceinline__ u128 shfl_xor(u128 v, int d) {
+  const u64 lo = __shfl_xor_sync(0xffffffffu, (u64)v, d), hi = __shfl_xor_sync(0xffffffffu, (u64)(v >> 64), d);
+  return ((u128)hi << 64) | lo;
+}
+__device__ __forceinline__ u64 shfl_xor(u64 v, int d) { return __shfl_xor_sync(0xffffffffu, v, d); }
+__device__ __forceinline__ double real(u128 v) { return (double)(u64)(v >> 64) * 18446744073709551616.0 + (double)(u64)v; }
+
+// f in [0, 1) as the integer m < 2^24 times 2^-e
+__device__ __forceinline__ uint32_t as_ratio(float f, int& e) {
+  const uint32_t b = __float_as_uint(f), x = b >> 23;
+  e = 150 - (x ? (int)x : 1);
+  return (b & 0x7fffffu) | (x ? 0x800000u : 0u);
+}
+
+constexpr double kSmpOne = 8796093022208.0;    // 2^43: 2^20 of them add up in 64 bits
+constexpr int kSmpLow = 41;                    // bits of a weight below that
+constexpr double kSmpFine = 65536.0;           // the histogram's steps are finer by this
+
+// sums of a part of a row: weights in two words, and how many equal the threshold
+struct Part {
+  u64 hi, lo, n;
+};
+__device__ __forceinline__ Part operator+(Part a, Part b) { return {a.hi + b.hi, a.lo + b.lo, a.n + b.n}; }
+__device__ __forceinline__ Part operator-(Part a, Part b) { return {a.hi - b.hi, a.lo - b.lo, a.n - b.n}; }
+__device__ __forceinline__ Part lane_of(Part v, int lane) {
+  return {__shfl_sync(0xffffffffu, v.hi, lane), __shfl_sync(0xffffffffu, v.lo, lane), __shfl_sync(0xffffffffu, v.n, lane)};
+}
+template <int N>
+__device__ __forceinline__ Part lane_scan(Part v) {      // inclusive, over N lanes
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int d = 1; d < N; d <<= 1) {
+    const Part o{__shfl_up_sync(0xffffffffu, v.hi, d), __shfl_up_sync(0xffffffffu, v.lo, d), __shfl_up_sync(0xffffffffu, v.n, d)};
+    if (lane >= d) v = v + o;
+  }
+  return v;
+}
+
 struct SmpShared {
-  double table[16];                         // 2^(j / 16) scaled by 2^S
-  u64 warp[kSmpWarps], warp2[kSmpWarps];
+  double table[16];                         // 2^(j / 16) scaled by 2^43
+  u64 warp[kSmpWarps], warp2[kSmpWarps], warp3[kSmpWarps];
   u64 slot[5][kSmpMaxCluster];              // one value from each CTA of the cluster
-  u64 res[3];                               // what one CTA found, pushed to all
+  u64 res[4];                               // what one CTA found, pushed to all
   u64 sure;                                 // the estimate decided the row
-  uint32_t bin[3][kSmpBins];                // a bin's sum in three words of 15 bits and what up to 2^17 additions carry
+  Part before;                              // what lies before the warp's part that holds the token
+  u128 target;                              // the token is the first whose running sum exceeds it
+  double log_z;
+  int where;                                // that warp, or -1: another CTA's
+  alignas(16) uint32_t bin[4][kSmpBins];    // a bin's sum in words of Row::limb bits and what the additions carry
   uint32_t count;                           // values of one bin in this CTA
   u64 list[kSmpThreads];                    // those of the cluster: weights, keys
   uint32_t list_key[kSmpThreads];
-  u64 red[1];                               // [kSmpBins / cluster size]: this CTA's share of the bins, summed over the cluster
 };
+// 64-bit weights are queued in bin[1], and the CTAs' structures lie at multiples of 128 bytes
+static_assert(offsetof(SmpShared, bin) % 16 == 0 && offsetof(SmpShared, list) % 8 == 0 && offsetof(SmpShared, target) % 16 == 0);
+static_assert(kSmpThreads * sizeof(u64) <= sizeof(uint32_t) * kSmpBins && kSmpWarps * 160 <= 4 * kSmpBins);
 
 template <typename T, int CS>
 struct Row {
@@ -134,11 +184,11 @@ struct Row {
   float base;          // the maximum, or the largest finite value where that is infinite
   float cut;           // values below weigh nothing
   double rate;         // 16 log2(e) / T
-  u64 one;             // 2^S
   double inv_t;
   SmpShared* s;
   uint32_t rank;
-  static constexpr uint32_t size = CS;
+  int limb;            // bits of a histogram word: 32 less what the slice's additions can carry
+  bool fine;           // weights go to the histogram in steps of 2^-59, else 2^-43
 
   // Comparisons take a NaN as it is: it is above nothing and equal to nothing, like the -inf it stands for.
   __device__ __forceinline__ float at(int i) const { return SmpType<T>::get(src[i]); }
@@ -147,11 +197,11 @@ struct Row {
     const uint32_t full = k << SmpType<T>::kGranule;
     return smp_value(full & 0x80000000u ? full : full | ((1u << SmpType<T>::kGranule) - 1));
   }
-  // exp((f - top) / T) * 2^S as an integer.  With x = 16 log2(e) (f - top) / T = 16 e + j + r, |r| <= 1/2, it is
+  // exp((f - top) / T) * 2^43.  With x = 16 log2(e) (f - top) / T = 16 e + j + r, |r| <= 1/2, it is
   // 2^e * table[j] * 2^(r / 16): twelve 64-bit operations and a 16-entry table whose entries lie in different banks;
-  // the Taylor polynomial of degree 5 leaves (ln 2 / 32)^6 / 6! = 2^-42.7.  f == top gives 2^S exactly.
+  // the Taylor polynomial of degree 5 leaves (ln 2 / 32)^6 / 6! = 2^-42.7.  f == top gives 2^43 exactly.
   // Without branches, so that several elements are in flight: what `cut` drops is computed and thrown away.
-  __device__ __forceinline__ u64 weight(float f) const {
+  __device__ __forceinline__ double scaled(float f) const {
     const double x = ((double)fminf(f, base) - (double)base) * rate;
     const double magic = 6755399441055744.0;                     // 1.5 * 2^52: the sum's low bits are round(x)
     const double xm = x + magic;
@@ -165,8 +215,27 @@ struct Row {
     const double tj = s->table[n & 15];
     y = fma(r * y, tj, tj);
     y = __hiloint2double(__double2hiint(y) + ((n >> 4) << 20), __double2loint(y));
-    y += 4503599627370496.0;                                     // 2^52: the low 52 bits are the rounded value
-    return f >= cut ? (u64)__double_as_longlong(y) & 0xfffffffffffffull : 0ull;
+    return f >= cut ? y : 0.0;
+  }
+  // that times 2^41, rounded, as hi 2^41 + lo with a signed lo: the rounded value and what is left of it, which is exact.
+  // Added to hi and lo as the bits of a double that has them in its low end, kHi and kLo above what they are.
+  static constexpr u64 kHi = 0x4330000000000000ull, kLo = 0x4338000000000000ull;     // 2^52, 1.5 * 2^52
+  static __device__ __forceinline__ void add_raw(double y, u64& hi, u64& lo) {
+    const double big = 4503599627370496.0, magic = 6755399441055744.0;
+    const double up = y + big;
+    hi += (u64)__double_as_longlong(up);
+    lo += (u64)__double_as_longlong(fma(y - (up - big), (double)(1ull << kSmpLow), magic));
+  }
+  static __device__ __forceinline__ u128 join(u64 hi, u64 lo) { return ((u128)hi << kSmpLow) + (u128)(__int128)(long long)lo; }
+  __device__ __forceinline__ u128 weight(float f) const {
+    u64 hi = 0, lo = 0;
+    add_raw(scaled(f), hi, lo);
+    return join(hi - kHi, lo - kLo);
+  }
+  // in the histogram's steps
+  __device__ __forceinline__ u64 binned(float f) const {
+    const double y = scaled(f);
+    return fine ? __double2ull_rn(y * kSmpFine) : (u64)__double_as_longlong(y + 4503599627370496.0) & 0xfffffffffffffull;
   }
   // coarse bin of a value, 0 = the highest: 1/64 of a logit each, the last takes the rest (and NaN)
   __device__ __forceinline__ int coarse(float f) const {
@@ -210,9 +279,10 @@ __device__ __forceinline__ double real(u64 v) { return __longlong_as_double((lon
 // the exponent t, three roundings of 2^-24, adds ln 2 * 3 * |t| * 2^-24 of the weight, for which sum w |t| is kept too:
 //   |error of any running sum| <= E = 2^-24 (7 Z + 2.1 sum w |t|).
 // A token whose running sums lie further than 2 E from u Z on both sides is the one that exact sums would choose;
-// else the row is decided by those.  Returns whether it is done.
+// else the row is decided by those.  Returns whether it is done.  A function of its own, so that what follows in the kernel
+// does not cost its loops registers (256 x 128256 f32 with min-p: 84 -> 80 us).
 template <typename T, int CS>
-__device__ bool estimate(Row<T, CS>& r, const SampleParams& p, int row, float least, float u) {
+__device__ __noinline__ bool estimate(Row<T, CS> r, const SampleParams& p, int row, float least, float u) {
   SmpShared& s = *r.s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const float rate = (float)(r.inv_t * 1.4426950408889634), base = r.base;
@@ -306,104 +376,149 @@ __device__ bool estimate(Row<T, CS>& r, const SampleParams& p, int row, float le
   return s.sure != 0;
 }
 
+// Counts fit 64 bits, sums of weights do not.
+template <bool WEIGHT> using Sum = std::conditional_t<WEIGHT, u128, u64>;
+
 // What is looked for: a sum of at least `target`, or, where that is 0, of at least `share` of (all - surplus).
+template <bool WEIGHT>
 struct Goal {
-  u64 target;
-  double share;
-  u64 surplus;
+  Sum<WEIGHT> target;
+  float share;         // in [0, 1)
+  Sum<WEIGHT> surplus;
 };
 
-// Looks for the bin in which the sum from bin 0 on reaches the goal: its index, the sum of the bins
-// before it and its own.  The bins of all CTAs of the cluster are added up first.
+// Looks for the bin in which the sum from bin 0 on reaches the goal: its index, how much of the goal the bins before
+// it leave to it, and (counts) what it holds, to res[] of every CTA.  The bins of all CTAs are added up first.
 template <bool WEIGHT, typename T, int CS>
-__device__ void find_bin(Row<T, CS>& r, Goal& goal, int& bin, u64& before, u64& inside) {
+__device__ __forceinline__ void find_bin(Row<T, CS>& r, const Goal<WEIGHT>& goal) {
   SmpShared& s = *r.s;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, limb = r.limb;
   constexpr int nb = kSmpBins / CS, per = (nb + kSmpThreads - 1) / kSmpThreads;
   cluster_sync_all();                                   // every CTA's bins are complete
-  u64 mine = 0;
-#pragma unroll
-  for (int e = 0; e < per; ++e) {
-    const int j = tid * per + e;
-    if (j >= nb) break;
-    const uint32_t from = smem_u32(&s.bin[0][r.rank * nb + j]);
-    constexpr int W = WEIGHT ? 3 : 1;
+  auto read = [&](int e, u64& lo, u64& hi) {            // this thread's e-th bin is lo + 2^(2 limb) hi
+    const uint32_t from = smem_u32(&s.bin[0][r.rank * nb + tid * per + e]);
+    constexpr int W = WEIGHT ? 4 : 1;
     uint32_t l[CS][W];                                  // all loads in flight before the first is used
 #pragma unroll
     for (uint32_t c = 0; c < CS; ++c)
 #pragma unroll
-      for (int w = 0; w < W; ++w) l[c][w] = ld_cluster_u32(mapa_cluster(from + w * kSmpBins * 4, c));
-    u64 v = 0;
+      for (int w = 0; w < W; ++w) l[c][w] = w == 3 && !r.fine ? 0 : ld_cluster_u32(mapa_cluster(from + w * kSmpBins * 4, c));
+    lo = hi = 0;
 #pragma unroll
-    for (int c = 0; c < CS; ++c)
+    for (int c = 0; c < CS; ++c) {
+      lo += l[c][0];
+      if constexpr (WEIGHT) {
+        lo += (u64)l[c][1] << limb;
+        hi += l[c][2] + ((u64)l[c][3] << limb);         // l[c][3] only where the steps are fine
+      }
+    }
+  };
+  u64 mine_lo = 0, mine_hi = 0;
 #pragma unroll
-      for (int w = 0; w < W; ++w) v += (u64)l[c][w] << (15 * w);
-    s.red[j] = v;
-    mine += v;
+  for (int e = 0; e < per; ++e) {
+    if (tid * per + e >= nb) break;
+    u64 lo, hi;
+    read(e, lo, hi);
+    mine_lo += lo;
+    mine_hi += hi;
   }
-  u64 total;
-  u64 end = block_scan(mine, s.warp, total);
-  r.push(0, total);
+  // in steps of 2^-43 a row's sum fits one word
+  const bool wide = WEIGHT && r.fine;
+  if (WEIGHT && !wide) { mine_lo += mine_hi << (2 * limb); mine_hi = 0; }
+  auto sum = [&](u64 low, u64 high) -> Sum<WEIGHT> {
+    if constexpr (WEIGHT) return ((u128)high << (2 * limb)) + low;
+    else return low;
+  };
+  u64 total_lo, total_hi = 0, end_lo = block_scan(mine_lo, s.warp, total_lo), end_hi = 0;
+  if (wide) end_hi = block_scan(mine_hi, s.warp2, total_hi);
+  r.push(0, total_lo);
+  if (wide) r.push(1, total_hi);
   cluster_sync_all();
-  u64 all = 0;
-  for (uint32_t c = 0; c < r.size; ++c) {
-    if (c < r.rank) end += s.slot[0][c];
-    all += s.slot[0][c];
+  Sum<WEIGHT> target = goal.target;
+  u64 all_lo = 0, all_hi = 0;
+  for (uint32_t c = 0; c < CS; ++c) {
+    const u64 v = s.slot[0][c], w = wide ? s.slot[1][c] : 0;
+    if (c < r.rank) { end_lo += v; end_hi += w; }
+    all_lo += v;
+    all_hi += w;
   }
-  if (goal.target == 0) {
-    const u64 z = all - goal.surplus;
-    const double want = ceil(goal.share * (double)z);
-    goal.target = want >= (double)z ? z : want < 1.0 ? 1 : (u64)want;
+  if constexpr (WEIGHT) {
+    if (target == 0) {
+      int shift;
+      const u128 want = (u128)(sum(all_lo, all_hi) - goal.surplus) * as_ratio(goal.share, shift);     // 2^79 * 2^24 at most
+      target = shift >= 128 ? want != 0 : (Sum<WEIGHT>)(want >> shift) + ((want & (((u128)1 << shift) - 1)) != 0);
+      if (target == 0) target = 1;
+    }
   }
-  u64 begin = end - mine;
-  if (begin < goal.target && goal.target <= end) {
-    int j = tid * per;
-    while (begin + s.red[j] < goal.target) begin += s.red[j++];
-    const u64 found[3] = {(u64)(r.rank * nb + j), begin, s.red[j]};
+  const Sum<WEIGHT> end = sum(end_lo, end_hi);
+  Sum<WEIGHT> begin = sum(end_lo - mine_lo, end_hi - mine_hi);
+  if (begin < target && target <= end) {
+    int e = 0;
+    Sum<WEIGHT> v = sum(mine_lo, mine_hi);
+    if constexpr (per > 1) {                            // one thread's: its bins once more
+      for (;; ++e) {
+        u64 lo, hi;
+        read(e, lo, hi);
+        v = sum(lo, hi);
+        if (target <= begin + v) break;
+        begin += v;
+      }
+    }
+    const Sum<WEIGHT> rest = target - begin;
+    const u64 found[3] = {(u64)(r.rank * nb + tid * per + e), (u64)rest, WEIGHT ? (u64)((u128)rest >> 64) : (u64)v};
 #pragma unroll
     for (int i = 0; i < 3; ++i)
 #pragma unroll
       for (uint32_t c = 0; c < CS; ++c) st_cluster_u64(mapa_cluster(smem_u32(&s.res[i]), c), found[i]);
   }
   cluster_sync_all();
-  bin = (int)s.res[0];
-  before = s.res[1];
-  inside = s.res[2];
-  __syncthreads();
+}
+template <bool WEIGHT>
+__device__ __forceinline__ Sum<WEIGHT> found_rest(const SmpShared& s) {
+  if constexpr (WEIGHT) return ((u128)s.res[2] << 64) | s.res[1];
+  else return s.res[1];
 }
 
+template <bool WEIGHT>
 __device__ __forceinline__ void clear_bins(SmpShared& s) {
-  for (int j = threadIdx.x; j < kSmpBins; j += kSmpThreads) s.bin[0][j] = s.bin[1][j] = s.bin[2][j] = 0;
+  for (int j = threadIdx.x; j < kSmpBins; j += kSmpThreads) {
+    s.bin[0][j] = 0;
+    if constexpr (WEIGHT) s.bin[1][j] = s.bin[2][j] = s.bin[3][j] = 0;
+  }
   __syncthreads();
 }
 // Adds without reading back: an atomic whose result nobody waits for costs a slot, not a round trip.
 template <bool WEIGHT>
-__device__ __forceinline__ void add_bin(SmpShared& s, int bin, u64 w) {
-  if (!WEIGHT) {
+__device__ __forceinline__ void add_bin(SmpShared& s, int limb, int bin, u64 w) {
+  if constexpr (!WEIGHT) {
     atomicAdd(&s.bin[0][bin], 1u);
-    return;
+  } else {
+    const uint32_t mask = (1u << limb) - 1, low = (uint32_t)w, high = (uint32_t)(w >> 32);
+    const uint32_t upper = limb >= 16 ? high >> (2 * limb - 32) : __funnelshift_r(low, high, 2 * limb);       // of 2^59 at most
+    atomicAdd(&s.bin[0][bin], low & mask);
+    atomicAdd(&s.bin[1][bin], __funnelshift_r(low, high, limb) & mask);
+    if (upper) {                                         // slices of 2^14: 2^-7 of the largest weight and more, or 2^-23
+      atomicAdd(&s.bin[2][bin], upper & mask);
+      if (upper >> limb) atomicAdd(&s.bin[3][bin], upper >> limb);
+    }
   }
-  const uint32_t a = (uint32_t)w & 0x7fffu, b = (uint32_t)(w >> 15) & 0x7fffu, c = (uint32_t)(w >> 30);
-  atomicAdd(&s.bin[0][bin], a);
-  atomicAdd(&s.bin[1][bin], b);
-  if (c) atomicAdd(&s.bin[2][bin], c);                   // 2^-14 of the largest weight and more: few
 }
 
 // The largest value (key K) with (count or weight of the values >= it) >= the goal, over the values that are not
-// below `least`: K, the sum over the values above it and over those equal to it.
+// below `least`; how much of the goal the values above it leave to those equal to it, and (counts) how many these are.
 template <bool WEIGHT, typename T, int CS>
-__device__ void find_threshold(Row<T, CS>& r, Goal& goal, float least, uint32_t& K, u64& above, u64& equal) {
+__device__ __forceinline__ void find_threshold(Row<T, CS>& r, const Goal<WEIGHT>& goal, float least, uint32_t& K, Sum<WEIGHT>& rest, u64& equals) {
   SmpShared& s = *r.s;
   const int tid = threadIdx.x;
-  clear_bins(s);
+  clear_bins<WEIGHT>(s);
 #pragma unroll 4
   for (int i = tid; i < r.n; i += kSmpThreads) {
     const float f = r.at(i);
     if (f < least) continue;
-    add_bin<WEIGHT>(s, r.coarse(f), WEIGHT ? r.weight(f) : 1);
+    add_bin<WEIGHT>(s, r.limb, r.coarse(f), WEIGHT ? r.binned(f) : 1);
   }
-  int coarse;
-  find_bin<WEIGHT>(r, goal, coarse, above, equal);
+  find_bin<WEIGHT>(r, goal);
+  const int coarse = (int)s.res[0];
   // keys that the coarse bin may hold, a little more on both sides than its rounding can reach
   const double step = 1.0 / 64, top = (double)r.top;
   const double slack = 1e-6 * (fabs(top) + (coarse + 1) * step);
@@ -431,7 +546,7 @@ __device__ void find_threshold(Row<T, CS>& r, Goal& goal, float least, uint32_t&
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         if (!in[e]) continue;
-        const u64 w = WEIGHT ? r.weight(f[e]) : 1;
+        const u64 w = WEIGHT ? r.binned(f[e]) : 1;
         if (!w) continue;
         const uint32_t at = atomicAdd(&s.count, 1u);
         if (at < kSmpThreads) {
@@ -461,11 +576,12 @@ __device__ void find_threshold(Row<T, CS>& r, Goal& goal, float least, uint32_t&
           st_cluster_u64(mapa_cluster(smem_u32(&s.list[first + tid]), c), w);
         }
       }
+      const Sum<WEIGHT> left = found_rest<WEIGHT>(s);
       cluster_sync_all();
       // eight lanes to each of this CTA's own values
       for (uint32_t e0 = 0; e0 < own; e0 += kSmpThreads / 8) {
         const uint32_t e = e0 + tid / 8, k = s.list_key[first + min(e, own - 1)];
-        u64 more = 0, same = 0;
+        Sum<WEIGHT> more = 0, same = 0;
 #pragma unroll 4
         for (uint32_t i = tid & 7; i < n; i += 8) {
           const u64 w = s.list[i];
@@ -475,11 +591,11 @@ __device__ void find_threshold(Row<T, CS>& r, Goal& goal, float least, uint32_t&
         }
 #pragma unroll
         for (int d = 4; d; d >>= 1) {
-          more += __shfl_xor_sync(0xffffffffu, more, d);
-          same += __shfl_xor_sync(0xffffffffu, same, d);
+          more += shfl_xor(more, d);
+          same += shfl_xor(same, d);
         }
-        if (above + more < goal.target && goal.target <= above + more + same && (tid & 7) == 0) {   // equal values all write the same
-          const u64 found[3] = {k, above + more, same};
+        if (more < left && left <= more + same && (tid & 7) == 0) {   // equal values all write the same
+          const u64 found[3] = {k, (u64)(left - more), WEIGHT ? (u64)((u128)(left - more) >> 64) : (u64)same};
 #pragma unroll
           for (int i = 0; i < 3; ++i)
 #pragma unroll
@@ -488,8 +604,8 @@ __device__ void find_threshold(Row<T, CS>& r, Goal& goal, float least, uint32_t&
       }
       cluster_sync_all();
       K = (uint32_t)s.res[0];
-      above = s.res[1];
-      equal = s.res[2];
+      rest = found_rest<WEIGHT>(s);
+      equals = s.res[2];
       __syncthreads();
       return;
     }
@@ -498,43 +614,73 @@ __device__ void find_threshold(Row<T, CS>& r, Goal& goal, float least, uint32_t&
   while (klo < khi) {
     const uint32_t span = khi - klo;
     const int bits = 32 - __clz(span), shift = bits > 11 ? bits - 11 : 0;
-    clear_bins(s);
+    const Goal<WEIGHT> left{found_rest<WEIGHT>(s), 0.f, 0};
+    clear_bins<WEIGHT>(s);
 #pragma unroll 4
     for (int i = tid; i < r.n; i += kSmpThreads) {
       const float f = r.at(i);
       if (r.coarse(f) != coarse || f < least) continue;
       const uint32_t k = r.key(f);
       if (k < klo || k > khi) continue;
-      const u64 w = WEIGHT ? r.weight(f) : 1;
-      if (w) add_bin<WEIGHT>(s, (int)((khi - k) >> shift), w);
+      const u64 w = WEIGHT ? r.binned(f) : 1;
+      if (w) add_bin<WEIGHT>(s, r.limb, (int)((khi - k) >> shift), w);
     }
-    int bin;
-    u64 before;
-    Goal rest{goal.target - above, 0.0, 0};
-    find_bin<WEIGHT>(r, rest, bin, before, equal);
-    above += before;
+    find_bin<WEIGHT>(r, left);
+    const int bin = (int)s.res[0];
     khi -= (uint32_t)bin << shift;
     const uint32_t low = khi - ((1u << shift) - 1);
     klo = low > klo && low <= khi ? low : klo;
     if (shift == 0) klo = khi;
   }
   K = khi;
+  rest = found_rest<WEIGHT>(s);
+  equals = s.res[2];
+  __syncthreads();
+}
+
+// the least n with n w >= rest, for a rest of up to 2^20 w
+__device__ __forceinline__ u64 how_many(u128 rest, u64 w) {
+  if (w == 0) return 1;
+  u64 n = (u64)(real(rest) / (double)w);
+  while (n > 1 && (u128)(n - 1) * w >= rest) --n;
+  while ((u128)n * w < rest) ++n;
+  return n;
+}
+
+// Top-p among the values that are not below `least`, of which the last `surplus` equal to it stay out: the threshold K
+// and how many of its equals stay in.  In steps of 2^-43 every weight is off by half a step, the difference of a running
+// sum and p Z so by less than V of them: a border further away than that is where it is in 64 bits too, else the steps
+// are made finer.
+template <typename T, int CS>
+__device__ __forceinline__ void find_top_p(Row<T, CS>& r, float p, float least, u64 surplus, int V, uint32_t& K, u64& allowed) {
+  for (r.fine = false;; r.fine = true) {
+    u128 rest;
+    u64 unused;
+    find_threshold<true>(r, Goal<true>{0, p, (u128)surplus * r.binned(least)}, least, K, rest, unused);
+    const float f = r.value(K);
+    const u64 w = r.binned(f), margin = (u64)V + 2;
+    allowed = how_many(rest, w);
+    if (r.fine) return;
+    const bool first = allowed == 1 && f == r.top;       // stays in whatever its predecessors, none, weigh
+    const u128 over = (u128)allowed * w - rest;          // w = 0: wraps, but then nothing is clear
+    if (w > margin && over > margin && (first || w - (u64)over > margin)) return;
+  }
 }
 
 // FILTERS: some row may have a top-k or top-p
 template <typename T, int CS, bool FILTERS>
-__global__ void __launch_bounds__(kSmpThreads, FILTERS ? 0 : 3) sample_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(kSmpThreads, FILTERS ? 2 : 3) sample_kernel(const SampleParams p) {
   extern __shared__ __align__(128) unsigned char smem[];
   SmpShared& s = *reinterpret_cast<SmpShared*>(smem);
   T* stage = reinterpret_cast<T*>(smem + p.stage_at);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  constexpr uint32_t size = CS;
   Row<T, CS> r;
   r.rank = CS == 1 ? 0 : cluster_ctarank();
   r.s = &s;
   const int row = blockIdx.x / CS;
   r.first = (int)r.rank * p.slice;
   r.n = max(0, min(p.slice, p.V - r.first));
+  r.limb = __clz(p.slice - 1);                           // slice <= 2^(32 - limb); 15 bits at V = 2^20
   const T* src = reinterpret_cast<const T*>(p.x) + (int64_t)row * p.ld + r.first;
   r.src = p.staged ? stage : src;
   const float t = p.t_row ? p.t_row[row] : p.t, pp = p.p_row ? p.p_row[row] : p.p;
@@ -603,20 +749,20 @@ __global__ void __launch_bounds__(kSmpThreads, FILTERS ? 0 : 3) sample_kernel(co
     }
     return;
   }
-  r.one = 1ull << p.scale;
   r.inv_t = 1.0 / (double)t;
   r.rate = r.inv_t * 23.083120654223415;                 // 16 log2(e)
-  // below max - 48 ln(2) T a weight rounds to zero
+  // below max - 85.5 ln(2) T a weight rounds to zero
   r.base = fminf(r.top, 3.402823466e38f);
-  r.cut = fmaxf((float)((double)r.top - 33.3 * (double)t), -3.402823466e38f);
-  if (tid < 16) s.table[tid] = exp2(tid / 16.0) * (double)r.one;
+  r.cut = fmaxf((float)((double)r.top - 59.3 * (double)t), -3.402823466e38f);
+  if (tid < 16) s.table[tid] = exp2(tid / 16.0) * kSmpOne;
   __syncthreads();
 
   const float u = u_row > 0.f ? u_row : 0.f;
   if (!FILTERS || (!(k > 0 && k < p.V) && !(pp < 1.f))) {
     // min-p as a limit of the logits: the least float that is not below max + T ln(min_p)
     const double limit = (double)r.top + (double)t * log((double)fmaxf(r_min_p, 0.f));
-    const float least = fmaxf(r_min_p > 0.f && r.top < INFINITY ? __double2float_ru(limit) : -INFINITY, r.cut);
+    const float cut = fmaxf((float)((double)r.top - 33.3 * (double)t), -3.402823466e38f);      // 2^-48 of the largest
+    const float least = fmaxf(r_min_p > 0.f && r.top < INFINITY ? __double2float_ru(limit) : -INFINITY, cut);
     if (estimate(r, p, row, least, u)) return;
   }
 
@@ -624,44 +770,38 @@ __global__ void __launch_bounds__(kSmpThreads, FILTERS ? 0 : 3) sample_kernel(co
   uint32_t K = 0;
   u64 allowed = ~0ull;
   if (FILTERS && k > 0 && k < p.V) {
-    u64 above, equal;
-    Goal goal{(u64)k, 0.0, 0};
-    find_threshold<false>(r, goal, -INFINITY, K, above, equal);
-    allowed = (u64)k - above;
+    u64 equals;
+    find_threshold<false>(r, Goal<false>{(u64)k, 0.f, 0}, -INFINITY, K, allowed, equals);
     if (pp < 1.f) {
-      const u64 equals = equal;
       uint32_t Kp;
-      Goal share{0, (double)fmaxf(pp, 0.f), (equals - allowed) * r.weight(r.value(K))};
-      find_threshold<true>(r, share, r.value(K), Kp, above, equal);
-      const u64 w = r.weight(r.value(Kp));
-      const u64 m = w ? (share.target - above + w - 1) / w : 1;
+      u64 m;
+      find_top_p(r, fmaxf(pp, 0.f), r.value(K), equals - allowed, p.V, Kp, m);
       if (Kp != K || m < allowed) allowed = m;
       K = Kp;
     }
   } else if (FILTERS && pp < 1.f) {
-    u64 above, equal;
-    Goal share{0, (double)fmaxf(pp, 0.f), 0};
-    find_threshold<true>(r, share, -INFINITY, K, above, equal);
-    const u64 w = r.weight(r.value(K));
-    allowed = w ? (share.target - above + w - 1) / w : 1;
+    find_top_p(r, fmaxf(pp, 0.f), -INFINITY, 0, p.V, K, allowed);
   }
 
   // ---- sums of what stays in, in the order of the vocabulary: a contiguous part for each warp
-  const u64 w_min = (u64)ceil((double)fmaxf(r_min_p, 0.f) * (double)r.one);
+  const double y_min = (double)fmaxf(r_min_p, 0.f) * kSmpOne;
   const bool filtered = FILTERS && allowed != ~0ull;
   const float fk = filtered ? r.value(K) : -INFINITY;    // above it all stay in, of its equals the first `allowed`
-  u64 w_eq = filtered ? r.weight(fk) : 0;
-  if (w_eq < w_min) w_eq = 0;
+  const u128 w_eq = filtered && r.scaled(fk) >= y_min ? r.weight(fk) : 0;
   const int part = (r.n + kSmpWarps * 32 - 1) / (kSmpWarps * 32) * 32;
   const int i0 = min(warp * part, r.n), i1 = min(i0 + part, r.n);
-  u64 sum = 0;
+  auto add = [&](float f, u64& hi, u64& lo) {
+    const double y = r.scaled(f);
+    r.add_raw(y >= y_min ? y : 0.0, hi, lo);
+  };
+  u64 hi = 0, lo = 0;
   uint32_t eq = 0;
   if (!filtered) {
 #pragma unroll 8
-    for (int i = i0 + lane; i < i1; i += 32) {
-      const u64 w = r.weight(r.at(i));
-      sum += w >= w_min ? w : 0;
-    }
+    for (int i = i0 + lane; i < i1; i += 32) add(r.at(i), hi, lo);
+    const u64 added = i1 > i0 + lane ? (i1 - i0 - lane + 31) / 32 : 0;
+    hi -= added * r.kHi;
+    lo -= added * r.kLo;
   } else {
     // few stay in: they are queued until there is one for every lane
     float* const queue = reinterpret_cast<float*>(s.bin) + warp * 160;
@@ -685,76 +825,115 @@ __global__ void __launch_bounds__(kSmpThreads, FILTERS ? 0 : 3) sample_kernel(co
       __syncwarp();
       while (n >= 32) {                                  // from the end, so that nothing has to move
         n -= 32;
-        const u64 w = r.weight(queue[n + lane]);
-        sum += w >= w_min ? w : 0;
+        add(queue[n + lane], hi, lo);
+        hi -= r.kHi;
+        lo -= r.kLo;
       }
       __syncwarp();
     }
-    const u64 w = lane < n ? r.weight(queue[lane]) : 0;
-    sum += w >= w_min ? w : 0;
+    if (lane < n) {
+      add(queue[lane], hi, lo);
+      hi -= r.kHi;
+      lo -= r.kLo;
+    }
   }
-  sum = warp_sum(sum);
+  hi = warp_sum(hi);
+  lo = warp_sum(lo);
   eq = __reduce_add_sync(0xffffffffu, eq);
   __syncthreads();
-  if (lane == 0) { s.warp[warp] = sum; s.warp2[warp] = eq; }
+  if (lane == 0) { s.warp[warp] = hi; s.warp2[warp] = eq; s.warp3[warp] = lo; }
   __syncthreads();
-  {
-    u64 a = 0, b = 0;
-#pragma unroll
-    for (int w = 0; w < kSmpWarps; ++w) { a += s.warp[w]; b += s.warp2[w]; }
-    r.push(1, a);
-    r.push(2, b);
+  // weight of a part, of its values equal to K the first `allowed`
+  auto weigh = [&](Part v) { return r.join(v.hi, v.lo) + (v.n < allowed ? v.n : allowed) * w_eq; };
+  // One warp for all: lane w has warp w's part, lane c CTA c's.
+  Part in_warp{0, 0, 0}, up_to_warp, in_cta;
+  if (warp == 0) {
+    if (lane < kSmpWarps) in_warp = {s.warp[lane], s.warp3[lane], s.warp2[lane]};
+    up_to_warp = lane_scan<kSmpWarps>(in_warp);
+    in_cta = lane_of(up_to_warp, kSmpWarps - 1);
+    r.push(1, in_cta.hi);
+    r.push(2, in_cta.n);
+    r.push(3, in_cta.lo);
   }
   cluster_sync_all();
-  auto kept = [&](u64 n) { return (n < allowed ? n : allowed) * w_eq; };   // weight of the first n values equal to K
-  u64 z = 0, n_eq = 0, mine = 0, mine_eq = 0;
-  for (uint32_t c = 0; c < size; ++c) {
-    if (c == r.rank) { mine = z; mine_eq = n_eq; }
-    z += s.slot[1][c];
-    n_eq += s.slot[2][c];
+  if (warp == 0) {
+    const Part up_to_cta = lane_scan<CS>(lane < CS ? Part{s.slot[1][lane], s.slot[3][lane], s.slot[2][lane]} : Part{0, 0, 0});
+    const u128 z = weigh(lane_of(up_to_cta, CS - 1));
+    const Part before_cta = lane_of(up_to_cta, r.rank) - in_cta;
+    u128 target = z - 1;
+    if (u < 1.f) {
+      int shift;
+      const u128 scaled = z * as_ratio(u, shift);        // 2^104 * 2^24 at most
+      target = shift >= 128 ? 0 : scaled >> shift;
+    }
+    const Part to = before_cta + up_to_warp, from = to - in_warp;
+    const bool here = lane < kSmpWarps && weigh(from) <= target && target < weigh(to);
+    if (here) s.before = from;
+    const unsigned which = __ballot_sync(0xffffffffu, here);
+    if (lane == 0) {
+      s.target = target;
+      s.log_z = log(real(z) / (kSmpOne * (double)(1ull << kSmpLow)));
+      s.where = __ffs(which) - 1;
+    }
   }
-  z += kept(n_eq);
-  const double at = (double)u * (double)z;
-  u64 target = at >= (double)z ? z - 1 : (u64)at;
-  if (target >= z) target = z - 1;
-  int where = -1;                                        // the warp's part that holds the token
-  for (int w = 0; w < kSmpWarps; ++w) {
-    const u64 a = s.warp[w], b = s.warp2[w];
-    const u64 begin = mine + kept(mine_eq), end = mine + a + kept(mine_eq + b);
-    if (begin <= target && target < end) { where = w; break; }
-    mine += a;
-    mine_eq += b;
+  __syncthreads();
+  auto choose = [&](int i, float f) {
+    p.token[row] = r.first + i;
+    if (p.logprob) p.logprob[row] = (float)((f == r.top ? 0.0 : ((double)f - (double)r.top) * r.inv_t) - s.log_z);
+  };
+  if (u == 0.f) {
+    // The first token that is kept and whose weight is not zero in 64 bits: below e^-745.13 it is.  Its index as the
+    // maximum of the complement.
+    u64 at = 0;
+    const double ln_min = r_min_p > 0.f ? log((double)r_min_p) : -INFINITY;
+    for (int i = tid; i < r.n; i += kSmpThreads) {
+      const float f = r.at(i);
+      const double e = f == r.top ? 0.0 : ((double)f - (double)r.top) * r.inv_t;
+      if (f >= fk && e > -745.13 && (f >= r.cut ? r.scaled(f) >= y_min : e >= ln_min)) { at = (uint32_t)~(uint32_t)(r.first + i); break; }
+    }
+    at = warp_max(at);
+    __syncthreads();
+    if (lane == 0) s.warp[warp] = at;
+    __syncthreads();
+    for (int w = 0; w < kSmpWarps; ++w) at = s.warp[w] > at ? s.warp[w] : at;
+    r.push(0, at);
+    cluster_sync_all();
+    for (uint32_t c = 0; c < CS; ++c) at = s.slot[0][c] > at ? s.slot[0][c] : at;
+    const int i = (int)~(uint32_t)at - r.first;
+    if (tid == 0 && i >= 0 && i < r.n) choose(i, r.at(i));
+    return;
   }
+  const int where = s.where;
   if (where < 0) return;                                 // another CTA's
+  const u128 target = s.target;
   // ---- that part once more, spread over the CTA: each thread a few neighbours
   const int j0 = min(where * part, r.n), j1 = min(j0 + part, r.n);
   const int per = (part + kSmpThreads - 1) / kSmpThreads;
   const int e0 = min(j0 + tid * per, j1), e1 = min(e0 + per, j1);
-  sum = 0;
-  eq = 0;
+  hi = lo = eq = 0;
   for (int i = e0; i < e1; ++i) {
     const float f = r.at(i);
     if (f == fk) ++eq;
     if (f > fk) {
-      const u64 w = r.weight(f);
-      if (w >= w_min) sum += w;
+      add(f, hi, lo);
+      hi -= r.kHi;
+      lo -= r.kLo;
     }
   }
   u64 unused;
-  const u64 sum_end = block_scan(sum, s.warp, unused), eq_end = block_scan(eq, s.warp2, unused);
-  mine += sum_end - sum;
-  mine_eq += eq_end - eq;
-  if (mine + kept(mine_eq) <= target && target < mine + sum + kept(mine_eq + eq)) {
+  const u64 hi_end = block_scan(hi, s.warp, unused), lo_end = block_scan(lo, s.warp3, unused), eq_end = block_scan(eq, s.warp2, unused);
+  Part mine = s.before + Part{hi_end - hi, lo_end - lo, eq_end - eq};
+  if (weigh(mine) <= target && target < weigh(mine + Part{hi, lo, eq})) {
     for (int i = e0; i < e1; ++i) {
       const float f = r.at(i);
-      if (f == fk) ++mine_eq;
+      if (f == fk) ++mine.n;
       if (f > fk) {
-        const u64 w = r.weight(f);
-        if (w >= w_min) mine += w;
+        add(f, mine.hi, mine.lo);
+        mine.hi -= r.kHi;
+        mine.lo -= r.kLo;
       }
-      if (mine + kept(mine_eq) > target) {
-        p.token[row] = r.first + i;
-        if (p.logprob) p.logprob[row] = (float)((f == r.top ? 0.0 : ((double)f - (double)r.top) * r.inv_t) - log((double)z / (double)r.one));
+      if (weigh(mine) > target) {
+        choose(i, f);
         break;
       }
     }
@@ -767,10 +946,9 @@ template <typename T, int CS, bool FILTERS>
 static int launch_sample_cluster(SampleParams& p, cudaStream_t st) {
   p.slice = ((p.V + CS - 1) / CS + 31) / 32 * 32;
   const int64_t bytes = (int64_t)p.slice * sizeof(T);
-  p.stage_at = (int)((FILTERS ? sizeof(SmpShared) + sizeof(u64) * (kSmpBins / CS) : offsetof(SmpShared, bin)) + 127) / 128 * 128;
+  p.stage_at = (int)((FILTERS ? sizeof(SmpShared) : offsetof(SmpShared, bin)) + 127) / 128 * 128;
   p.staged = bytes <= kSmpMaxSmem - p.stage_at;
   const int smem = p.stage_at + (p.staged ? (int)bytes : 0);
-  p.scale = p.V <= (1 << 19) ? 44 : 43;
   auto kern = sample_kernel<T, CS, FILTERS>;
   cudaError_t e = ensure_dynamic_smem(kern, kSmpMaxSmem);
   if (e != cudaSuccess) return set_cuda_error("sample_tokens shared memory", e);

@@ -347,8 +347,10 @@ ARKE_B200_API int arke_b200_paged_gqa_fwd(const void* q, int64_t q_stride_token,
  *   token  = the first kept index i, in vocabulary order, with sum_{j <= i, kept} w_j > u * Z, Z the sum
  *            of what is kept;  logprob [B] (may be NULL) = log(w_token / Z).
  * temperature <= 0: the arg max (lowest index), logprob 0.  A NaN logit counts as -inf, which is never
- * chosen; a row of -inf alone gives token -1, logprob -inf.  u outside [0, 1) is clamped.  Decisions are
- * those of 64-bit arithmetic and do not depend on how the work is split.
+ * chosen; a row of -inf alone gives token -1, logprob -inf.  u outside [0, 1) is clamped; at u = 0 the first
+ * kept token whose weight is not zero in 64 bits is chosen.  Decisions are those of 64-bit arithmetic and do not
+ * depend on how the work is split: a weight is off by 2^-42 of itself and 2^-85 of the largest, where top_p
+ * looks for its border by 2^-60 of the largest.
  * A value for all rows must be in range (temperature, top_k, top_p >= 0, min_p in [0, 1]); of arrays, negative entries
  * count as 0.  Each parameter is a value for all rows, or a device array [B] (fp32; top_k int32) where it is not NULL. */
 ARKE_B200_API int arke_b200_sample_tokens(const void* logits, int dtype, int64_t ld, int64_t B, int64_t V,
