@@ -278,6 +278,8 @@ __device__ __forceinline__ double real(u64 v) { return __longlong_as_double((lon
 // their error: ex2 is good to 2^-22, eight weights are added in a tree of depth three before they go to 64 bits, and
 // the exponent t, three roundings of 2^-24, adds ln 2 * 3 * |t| * 2^-24 of the weight, for which sum w |t| is kept too:
 //   |error of any running sum| <= E = 2^-24 (7 Z + 2.1 sum w |t|).
+// The hundredth that is added to E covers what `least` leaves out, 2^20 weights of 2^-48 at most; so a first token is
+// not sure either while u Z lies within that of zero.
 // A token whose running sums lie further than 2 E from u Z on both sides is the one that exact sums would choose;
 // else the row is decided by those.  Returns whether it is done.  A function of its own, so that what follows in the kernel
 // does not cost its loops registers (256 x 128256 f32 with min-p: 84 -> 80 us).
@@ -360,7 +362,7 @@ __device__ __noinline__ bool estimate(Row<T, CS> r, const SampleParams& p, int r
         const float f = r.at(e);
         const double next = mine + (double)weight(f, t);
         if (target < next) {
-          if (next - target > 2.0 * bound && (mine == 0.0 || target - mine > 2.0 * bound)) {
+          if (next - target > 2.0 * bound && target - mine > 2.0 * bound) {
             p.token[row] = r.first + e;
             if (p.logprob) p.logprob[row] = (float)((f == r.top ? 0.0 : ((double)f - (double)r.top) * r.inv_t) - log(total));
 #pragma unroll

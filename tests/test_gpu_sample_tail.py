@@ -119,3 +119,24 @@ def test_the_number_zero_chooses_the_first_kept_token(f, t):
     p32, m32 = float(torch.tensor(f.get("top_p", 1.0))), float(torch.tensor(f.get("min_p", 0.0)))
     want = [oracle.sample(r.numpy(), 0.0, t, f.get("top_k", 0), p32, m32)[0] for r in x]
     assert got.tolist() == want
+
+
+@pytest.mark.parametrize("V, level", [(4096, 60.0), (128256, 49.5), (1 << 20, 49.5), (50257, 300.0)])
+@pytest.mark.parametrize("how", ["numbers", "rows", "many rows"])
+def test_small_numbers_in_front_of_a_peak(V, level, how):
+    """No filter, all the weight in the last token, and a number that falls into the tail in front of it: u = 0, and the
+    middle of the tail's share, which is 2^-30 of the whole at most and far from every border."""
+    n = 300 if how == "many rows" else 2                    # the kernel for batches without filters starts at some 40 rows
+    x = tail(V, level)
+    w = math.exp(float(x[0]))
+    middle = (V // 2 + 0.5) * w                            # of a whole that is 1 to 2^-29
+    u = torch.tensor([0.0, middle], dtype=torch.float32)
+    j = expected(x, u.tolist(), np.arange(V))
+    kw = {}
+    if how == "rows":
+        kw = dict(temperature=rows(1.0, n), top_k=rows(0, n, torch.int32), top_p=rows(1.0, n), min_p=rows(0.0, n))
+    us = u.cuda().repeat((n + 1) // 2)[:n]
+    got = _ops().sample_tokens(x.cuda().expand(n, V).contiguous(), us, **kw).cpu()
+    assert (got[0::2] == 0).all()
+    if middle >= V * 2.0 ** -80:                            # within what running sums resolve
+        assert j[1] is not None and (got[1::2] == j[1]).all()
