@@ -761,8 +761,9 @@ __global__ void __launch_bounds__(kSmpThreads, FILTERS ? 2 : 3) sample_kernel(co
 
   const float u = u_row > 0.f ? u_row : 0.f;
   if (!FILTERS || (!(k > 0 && k < p.V) && !(pp < 1.f))) {
-    // min-p as a limit of the logits: the least float that is not below max + T ln(min_p)
-    const double limit = (double)r.top + (double)t * log((double)fmaxf(r_min_p, 0.f));
+    // min-p as a limit of the logits: the least float that is not below max + T ln(min_p), less what the exponential
+    // of 64 bits rounds up to min_p (2^-54, for min_p = 1 at temperatures that leave nothing of the differences)
+    const double limit = (double)r.top + (double)t * (log((double)fmaxf(r_min_p, 0.f)) - 5.551115123125783e-17);
     const float cut = fmaxf((float)((double)r.top - 33.3 * (double)t), -3.402823466e38f);      // 2^-48 of the largest
     const float least = fmaxf(r_min_p > 0.f && r.top < INFINITY ? __double2float_ru(limit) : -INFINITY, cut);
     if (estimate(r, p, row, least, u)) return;

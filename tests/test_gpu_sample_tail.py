@@ -140,3 +140,17 @@ def test_small_numbers_in_front_of_a_peak(V, level, how):
     assert (got[0::2] == 0).all()
     if middle >= V * 2.0 ** -80:                            # within what running sums resolve
         assert j[1] is not None and (got[1::2] == j[1]).all()
+
+
+@pytest.mark.parametrize("n", [4, 400])
+@pytest.mark.parametrize("f", [dict(), dict(top_k=999), dict(top_p=0.999999)], ids=str)
+def test_min_p_of_one_keeps_what_64_bits_cannot_tell_from_the_largest(n, f):
+    """At a temperature of 1e30 every weight is 1 in 64 bits, and 1 >= min_p: the same with and without other filters."""
+    V = 1000
+    x = torch.randn(V, generator=torch.Generator().manual_seed(1))
+    order = np.arange(V)
+    kept = f.get("top_k", math.ceil(float(torch.tensor(f.get("top_p", 1.0))) * V))      # of equal weights
+    order = np.sort(np.lexsort((order, -x.double().numpy()))[:kept])
+    u = (torch.arange(n) + 0.25) / n
+    got = _ops().sample_tokens(x.cuda().expand(n, V).contiguous(), u.cuda(), temperature=1e30, min_p=1.0, **f).cpu().tolist()
+    assert got == [int(order[int(float(v) * len(order))]) for v in u]
