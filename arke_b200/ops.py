@@ -558,9 +558,10 @@ def paged_gqa_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     ``j <= kv_len - n + i``, else all.  ``shared_prefix``: the first so many positions are the same for every
     sequence; their whole pages are read through ``block_table[0]``, once for the batch where that pays (of a page that
     the prefix fills in part every sequence has its own).  A row that sees nothing, and a row behind
-    ``cu_q[B]``, gives ``o = 0``, ``lse = -inf``; a page or length outside its range makes the rows that need it NaN
-    and sets status code 8.  ``workspace``: uint8, :func:`paged_gqa_workspace_bytes` long; calls that may overlap need
-    one each.
+    ``cu_q[B]``, gives ``o = 0``, ``lse = -inf``.  Where a page is outside its range the rows that see it are NaN, and
+    other rows of that sequence may be (of the batch, in a shared prefix); where a length is, every row of that sequence
+    is; both set status code 8.  ``workspace``: uint8, :func:`paged_gqa_workspace_bytes` long; calls that may overlap
+    need one each.
     """
     dev = _same_device(q, k_cache, v_cache, block_table, kv_lens, cu_q, workspace)
     if q.dtype != k_cache.dtype:

@@ -326,8 +326,9 @@ ARKE_B200_API int arke_b200_qkv_rope_paged_append(const void* qkv, int64_t ld, c
  *   shared_prefix: the first positions [0, shared_prefix) of every sequence are the same.  Their whole
  *   pages are read through sequence 0's row of the block table, and once for the whole batch where that
  *   pays; of a page that the prefix fills in part every sequence has its own.  0 = nothing shared.
- *   A page, or a length, outside its range: every row of that sequence (of the batch, when it lies in
- *   the shared prefix) is NaN, status code 8.
+ *   A page outside its range: the rows that see one of its positions are NaN, o and lse, and other rows of that
+ *   sequence may be (of the batch, when it lies in the shared prefix).  A length outside its range: every row of
+ *   that sequence is NaN.  Both set status code 8.
  *   workspace: arke_b200_paged_gqa_workspace(...) bytes, 256-byte aligned; contents need no
  *   initialisation and nothing is kept in it between calls; calls that may overlap need one each. */
 ARKE_B200_API size_t arke_b200_paged_gqa_workspace(int64_t T, int64_t batch, int64_t Hq, int64_t Hkv, int64_t D,
