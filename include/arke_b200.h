@@ -94,7 +94,7 @@ ARKE_B200_API int arke_b200_selftest_bounds_check(void* stream);
  *                   tiles; 0 = default: those tiles are cut into 2 or 4 narrower units along N
  *                   so that they spread over more CTA pairs
  *   "paged_prefix_kb" KB of re-read keys and values from which on a shared prefix of paged_gqa_fwd is
- *                   computed apart, once for all sequences (0 = default, 65536); set it before the
+ *                   computed apart, once for all sequences (0 = default, 40960); set it before the
  *                   workspace is asked for
  * Results do not depend on the gemm options; paged_prefix_kb changes in which order partial sums meet.
  * get_option returns -1 for an unknown name. */
