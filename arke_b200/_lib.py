@@ -29,13 +29,14 @@ ERR_NAMES = {
 class PagedKV(ctypes.Structure):
     """``arke_b200_paged_kv`` (include/arke_b200.h)."""
     # the same layout for struct.pack, which fills it in a third of the time: bytes serve as the pointer argument
-    packer = struct.Struct("@2P10qP2q2Pqi4x")
+    packer = struct.Struct("@2P10qP2q2Pq2i")
     _fields_ = [("k", c_void_p), ("v", c_void_p),
                 ("k_stride_page", c_int64), ("k_stride_head", c_int64), ("k_stride_row", c_int64),
                 ("v_stride_page", c_int64), ("v_stride_head", c_int64), ("v_stride_row", c_int64),
                 ("num_pages", c_int64), ("page_size", c_int64), ("heads", c_int64), ("head_dim", c_int64),
                 ("block_table", c_void_p), ("ld_table", c_int64), ("max_pages", c_int64),
-                ("kv_lens", c_void_p), ("cu_q", c_void_p), ("batch", c_int64), ("dtype", ctypes.c_int32)]
+                ("kv_lens", c_void_p), ("cu_q", c_void_p), ("batch", c_int64), ("dtype", ctypes.c_int32),
+                ("max_new", ctypes.c_int32)]
 
 
 class ArkeB200Error(RuntimeError):

@@ -21,6 +21,7 @@ struct PagedKV {
   const int* cu;
   int max_pages, num_pages, page_size;
   int B, uniform, T;       // T: query rows of the call, those behind the last sequence included
+  int max_new;             // most query rows of a sequence as the caller knows it, 0 = unknown
   int Hkv;
   int64_t k_ext, v_ext;    // elements the caches span (checked build)
 };

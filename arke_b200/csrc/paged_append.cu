@@ -277,6 +277,7 @@ int check_paged(const char* op, const arke_b200_paged_kv* d, int64_t T, int64_t 
   p.page_size = (int)d->page_size;
   p.B = (int)d->batch;
   p.T = (int)T;
+  p.max_new = d->max_new > 0 ? d->max_new : 0;
   p.uniform = d->batch > 0 ? (int)(T / d->batch) : 0;
   p.Hkv = (int)d->heads;
   if (d->num_pages > 0) {

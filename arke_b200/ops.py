@@ -466,7 +466,7 @@ _PACK_KV = _lib.PagedKV.packer.pack
 
 
 def _paged_kv(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor,
-              cu_q: Optional[torch.Tensor], T: int, Hq: int) -> Tuple[bytes, int, int, int]:
+              cu_q: Optional[torch.Tensor], T: int, Hq: int, max_new: int = 0) -> Tuple[bytes, int, int, int]:
     """Checks a cache description and packs it for the C ABI → (``arke_b200_paged_kv``, B, Hkv, D)."""
     dt = k_cache.dtype
     if dt not in (torch.bfloat16, torch.float16) or v_cache.dtype != dt:
@@ -499,7 +499,7 @@ def _paged_kv(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tab
     elif ldt < width:
         raise _lib.UnsupportedError(-3, f"{name}: block_table rows must not overlap")
     return (_PACK_KV(k_cache.data_ptr(), v_cache.data_ptr(), ksp, ksh, ksr, vsp, vsh, vsr, P, page, Hkv, D, block_table.data_ptr(), ldt,
-                     width, kv_lens.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(), B, _DT[dt]), B, Hkv, D)
+                     width, kv_lens.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(), B, _DT[dt], max_new), B, Hkv, D)
 
 
 def qkv_rope_paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -550,7 +550,8 @@ def paged_gqa_workspace_bytes(T: int, B: int, Hq: int, Hkv: int, D: int, shared_
 
 def paged_gqa_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor,
                   cu_q: Optional[torch.Tensor] = None, shared_prefix: int = 0, causal: bool = True,
-                  softmax_scale: Optional[float] = None, return_lse: bool = True, workspace: Optional[torch.Tensor] = None):
+                  softmax_scale: Optional[float] = None, return_lse: bool = True, workspace: Optional[torch.Tensor] = None,
+                  max_new: int = 0):
     """:func:`gqa_fwd` of a ragged batch over a paged cache: ``q [T,Hq,D]`` → ``o [T,Hq,D]`` and ``lse [T,Hq]`` (fp32).
 
     Caches, ``block_table``, ``kv_lens`` and ``cu_q`` as in :func:`qkv_rope_paged_append` (``D`` 64 or 128).  The
@@ -561,7 +562,9 @@ def paged_gqa_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     ``cu_q[B]``, gives ``o = 0``, ``lse = -inf``.  Where a page is outside its range the rows that see it are NaN, and
     other rows of that sequence may be (of the batch, in a shared prefix); where a length is, every row of that sequence
     is; both set status code 8.  ``workspace``: uint8, :func:`paged_gqa_workspace_bytes` long; calls that may overlap
-    need one each.
+    need one each.  ``max_new``: the most tokens that a sequence has, where the caller knows it (0: unknown).  With
+    ``cu_q`` it chooses the kernels, never the result: without it a prompt in a batch of mostly empty slots goes the way
+    of single tokens.
     """
     dev = _same_device(q, k_cache, v_cache, block_table, kv_lens, cu_q, workspace)
     if q.dtype != k_cache.dtype:
@@ -569,7 +572,9 @@ def paged_gqa_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     if q.dim() != 3:
         raise _lib.UnsupportedError(-3, "paged_gqa_fwd: q must be [T, Hq, D]")
     T, Hq, D = q.shape
-    kv, B, Hkv, Dk = _paged_kv("paged_gqa_fwd", k_cache, v_cache, block_table, kv_lens, cu_q, T, Hq)
+    if not 0 <= max_new <= 0x7fffffff:
+        raise _lib.ArkeB200Error(-1, f"paged_gqa_fwd: max_new must be a number of tokens, got {max_new}")
+    kv, B, Hkv, Dk = _paged_kv("paged_gqa_fwd", k_cache, v_cache, block_table, kv_lens, cu_q, T, Hq, max_new)
     if Dk != D:
         raise _lib.UnsupportedError(-3, f"paged_gqa_fwd: q has head_dim {D}, the caches {Dk}")
     st, sh, s1 = q.stride()
@@ -595,12 +600,12 @@ def paged_gqa_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
 def qkv_rope_paged_attention(x: torch.Tensor, w_qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_cache: torch.Tensor,
                              v_cache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor, Hq: int,
                              cu_q: Optional[torch.Tensor] = None, shared_prefix: int = 0, w_layout: str = "kn",
-                             return_lse: bool = False):
+                             return_lse: bool = False, max_new: int = 0):
     """:func:`qkv_rope_attention` for the next tokens of sequences in a paged cache: ``x [T, hidden]`` times ``w_qkv``,
     one :func:`qkv_rope_paged_append`, then :func:`paged_gqa_fwd`.  Returns ``O [T,Hq,D]`` (and ``lse``)."""
     qkv = matmul(x, w_qkv, b_layout=w_layout)
     q = qkv_rope_paged_append(qkv, cos, sin, k_cache, v_cache, block_table, kv_lens, Hq, cu_q=cu_q)
-    return paged_gqa_fwd(q, k_cache, v_cache, block_table, kv_lens, cu_q=cu_q, shared_prefix=shared_prefix, return_lse=return_lse)
+    return paged_gqa_fwd(q, k_cache, v_cache, block_table, kv_lens, cu_q=cu_q, shared_prefix=shared_prefix, return_lse=return_lse, max_new=max_new)
 
 
 # ---------------------------------------------------------------------------------------------

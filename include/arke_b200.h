@@ -285,7 +285,10 @@ ARKE_B200_API int arke_b200_fused_linear_ce_backward(const void* x, const void* 
  *   cu_q       [batch + 1] int32, non-decreasing from 0: sequence b owns the query rows
  *              [cu_q[b], cu_q[b + 1]); NULL: T / batch rows each.  Rows from cu_q[batch] to T belong to
  *              no sequence: their outputs are zero.  The tokens of a sequence are its last ones:
- *              row i of n has position kv_lens[b] - n + i.
+ *              row i of n has position kv_lens[b] - n + i;
+ *   max_new    no less than the longest sequence's query rows, or 0 if unknown.  Only paged_gqa_fwd's choice of
+ *              kernels goes by it, and only with cu_q: results are right whatever it says.  Unknown, every
+ *              sequence is taken to have a row, which a batch of mostly empty slots pays for.
  * A page outside [0, num_pages), a length below 0 or beyond max_pages * page_size, or (append) a
  * position below 0 or outside the cos / sin tables sets status code 8; nothing is read or written there. */
 typedef struct {
@@ -300,6 +303,7 @@ typedef struct {
   const int32_t* cu_q;
   int64_t batch;
   int32_t dtype;
+  int32_t max_new;
 } arke_b200_paged_kv;
 
 /* qkv_rope_split for a paged cache: qkv [T, ld] holds, per token, Hq query heads, then the key heads,

@@ -35,3 +35,77 @@ def test_rows_that_see_a_missing_page_are_nan(new, ctx, Hq, Hkv, where):
     gone = torch.isnan(o)
     assert (gone[:new][~sees] | right[:new][~sees]).all() and right[new:].all() and torch.isfinite(lse[new:]).all()
     assert torch.equal(gone.all(2), gone.any(2)) and torch.equal(torch.isnan(lse), gone.all(2))      # a row is NaN as a whole
+
+
+PADDED = [  # new tokens of each slot, lengths, heads, head_dim, page
+    ([0] * 300 + [200] + [0] * 99, [40] * 300 + [333] + [7] * 99, 8, 2, 64, 16),          # one prompt, 399 empty slots
+    ([0] * 20 + [70] + [0] * 60 + [1, 1, 3] + [0] * 50, [5] * 20 + [70] + [0] * 60 + [90, 31, 3] + [64] * 50, 4, 4, 128, 32),
+    ([64] + [0] * 64, [500] + [0] * 64, 8, 1, 64, 8),
+    ([0] * 700, [9] * 700, 4, 2, 64, 16),                                                  # nobody has a token
+]
+
+
+@pytest.mark.parametrize("case", PADDED, ids=lambda c: f"{sum(c[0])}tok{len(c[0])}slots")
+@pytest.mark.parametrize("tag", ["bf16", "f16"])
+@pytest.mark.parametrize("prefix", [0, 32])
+@pytest.mark.parametrize("told", ["nothing", "the longest", "too much", "too little"])
+def test_more_empty_sequences_than_tokens(case, tag, prefix, told):
+    """A batch of fixed slots, most without a token: the same rows as without the empty ones, rows behind the last are 0,
+    whatever the caller says of the longest sequence."""
+    new, lens, Hq, Hkv, D, page = case
+    if prefix:
+        lens = [n + prefix for n in lens]
+    dt = {"bf16": torch.bfloat16, "f16": torch.float16}[tag]
+    ops = _ops()
+    k, v, table = make_cache(lens, Hkv, D, page, dt, "hnd", 9, prefix)
+    cu = [0]
+    for n in new:
+        cu.append(cu[-1] + n)
+    T = cu[-1] + 3
+    q = (torch.randn(T, Hq, D, generator=torch.Generator().manual_seed(3)) * 1.5).to(dt)
+    with ops.options(paged_prefix_kb=1):
+        o, lse = ops.paged_gqa_fwd(q.cuda(), k.cuda(), v.cuda(), table.cuda(), _i32(lens).cuda(), cu_q=_i32(cu).cuda(), shared_prefix=prefix,
+                                   max_new={"nothing": 0, "the longest": max(new), "too much": 1 << 30, "too little": 1}[told])
+    o64, lse64 = oracle.paged_attention(q, k, v, table, lens, cu, prefix)
+    assert within_weights(o, o64, q, k, v, table, lens, cu, prefix, True)
+    seen = torch.isfinite(lse64)
+    assert torch.equal(torch.isfinite(lse.cpu()), seen) and (o.cpu()[~seen] == 0).all() and not seen[cu[-1]:].any()
+    assert ((lse.cpu().double() - lse64)[seen].abs() <= 2.0 ** -16 + 2.0 ** -23 * lse64[seen].abs()).all()
+    assert ops.kernel_status() == 0
+
+
+def within_weights(o, o64, q, k, v, table, lens, cu, prefix, causal):
+    """Half a step of the result; and of the weights, which may be rounded to 16 bits before they meet the values, half a
+    step of each (of 2^-25 at least where f16 has no normal numbers; the largest is 1 or more), and 2^-15 of each for
+    scores and sums in fp32 (a score below 2^6 is off by 2^-17, its weight and their sum by 2^-16 at most): the error of
+    a column is that share of sum_j p_j |v_j|, which is the same attention over |v|."""
+    dt = q.dtype
+    mean, _ = oracle.paged_attention(q, k, v.abs(), table, lens, cu, prefix, causal)
+    eps = torch.finfo(dt).eps
+    tol = eps / 2 * o64.abs() + (eps / 2 + 2.0 ** -15) * mean
+    if dt == torch.float16:
+        tol = tol + max(lens) * 2.0 ** -25 * v.double()[torch.isfinite(v)].abs().max()
+    return ((o.cpu().double() - o64).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("G", [1, 4, 7])
+def test_offsets_and_the_longest_sequence_choose_the_same_kernels_as_a_uniform_batch(G):
+    """Two sequences of 30 tokens: with cu_q and their length the call does what it does without cu_q, bit for bit."""
+    Hkv, D, page, dt, lens = 2, 64, 16, torch.bfloat16, [500, 333]
+    ops = _ops()
+    k, v, table = make_cache(lens, Hkv, D, page, dt, "hnd", 4)
+    q = torch.randn(60, Hkv * G, D, generator=torch.Generator().manual_seed(8)).to(dt).cuda()
+    args = (q, k.cuda(), v.cuda(), table.cuda(), _i32(lens).cuda())
+    o, lse = ops.paged_gqa_fwd(*args)
+    o2, lse2 = ops.paged_gqa_fwd(*args, cu_q=_i32([0, 30, 60]).cuda(), max_new=30)
+    assert torch.equal(o, o2) and torch.equal(lse, lse2) and ops.kernel_status() == 0
+
+
+def test_refusals_of_the_longest_sequence():
+    from arke_b200 import _lib
+    k = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16, device="cuda")
+    table, lens = torch.zeros(2, 2, dtype=torch.int32, device="cuda"), _i32([5, 6]).cuda()
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16, device="cuda")
+    for bad in (-1, 1 << 31):
+        with pytest.raises(_lib.ArkeB200Error):
+            _ops().paged_gqa_fwd(q, k, k, table, lens, max_new=bad)
