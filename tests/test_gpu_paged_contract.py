@@ -1,12 +1,10 @@
 """GPU: what paged attention promises beyond its results — broken tables, padded batches, the bound of its error — against
 64-bit restatements."""
-import math
-
 import pytest
 import torch
 
 from oracle import serving as oracle
-from test_gpu_paged import _i32, _ops, make_cache, o_tolerance, to_gpu
+from test_gpu_paged import ATTEND, TILES, _i32, _ops, make_cache, o_tolerance, prefix_units, to_gpu  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -109,3 +107,41 @@ def test_refusals_of_the_longest_sequence():
     for bad in (-1, 1 << 31):
         with pytest.raises(_lib.ArkeB200Error):
             _ops().paged_gqa_fwd(q, k, k, table, lens, max_new=bad)
+
+
+@pytest.mark.parametrize("case", ATTEND + TILES, ids=lambda c: f"{len(c[0])}seq{sum(c[0])}tok{c[2]}/{c[3]}x{c[4]}p{c[5]}s{c[7]}")
+@pytest.mark.parametrize("tag", ["bf16", "f16"])
+def test_error_is_within_the_weights_rounding(case, tag, prefix_units):
+    """Every column within what the rounding of the weights can move it, not only within what it moves the largest value."""
+    new, lens, Hq, Hkv, D, page, layout, prefix, causal = case
+    if prefix == 0 and prefix_units == "merged":
+        pytest.skip("no prefix")
+    dt = {"bf16": torch.bfloat16, "f16": torch.float16}[tag]
+    k, v, table = make_cache(lens, Hkv, D, page, dt, layout, len(new) * 5 + D, prefix)
+    cu = [0]
+    for n in new:
+        cu.append(cu[-1] + n)
+    q = (torch.randn(cu[-1], Hq, D, generator=torch.Generator().manual_seed(12)) * 1.5).to(dt)
+    o64, _ = oracle.paged_attention(q, k, v, table, lens, cu, prefix, causal)
+    args = (q.cuda(), to_gpu(k), to_gpu(v), table.cuda(), _i32(lens).cuda())
+    for max_new in (0, max(new)):
+        o, _ = _ops().paged_gqa_fwd(*args, cu_q=_i32(cu).cuda(), shared_prefix=prefix, causal=causal, max_new=max_new)
+        assert within_weights(o, o64, q, k, v, table, lens, cu, prefix, causal)
+    assert _ops().kernel_status() == 0
+
+
+def test_error_of_long_sequences_is_within_the_weights_rounding():
+    """Thousands of keys, where the result is small beside the largest value: tiles in parts, and tiles beside streamed keys."""
+    Hq, Hkv, D, page, dt = 8, 2, 64, 32, torch.bfloat16
+    g = torch.Generator().manual_seed(7)
+    for new, lens, prefix in [([40, 3], [5000, 3000], 0), ([1] * 24, [2048 + 100 * (b + 1) for b in range(24)], 2048)]:
+        k, v, table = make_cache(lens, Hkv, D, page, dt, "hnd", 13, prefix)
+        cu = [0]
+        for n in new:
+            cu.append(cu[-1] + n)
+        q = (torch.randn(cu[-1], Hq, D, generator=g) * 1.5).to(dt)
+        o64, _ = oracle.paged_attention(q, k, v, table, lens, cu, prefix)
+        with _ops().options(paged_prefix_kb=1):
+            o, _ = _ops().paged_gqa_fwd(q.cuda(), k.cuda(), v.cuda(), table.cuda(), _i32(lens).cuda(), cu_q=_i32(cu).cuda(),
+                                        shared_prefix=prefix, max_new=max(new))
+        assert within_weights(o, o64, q, k, v, table, lens, cu, prefix, True)
