@@ -26,7 +26,14 @@ struct PagedKV {
   int64_t k_ext, v_ext;    // elements the caches span (checked build)
 };
 
-__device__ __forceinline__ int seq_begin(const PagedKV& p, int b) { return p.cu ? p.cu[b] : b * p.uniform; }
+// Entries of the batch's description (the bounds are the checked build's).
+__device__ __forceinline__ int cu_at(const PagedKV& p, int b) { return ARKE_CHK(b, b, p.B + 1) ? p.cu[b] : 0; }
+__device__ __forceinline__ int len_at(const PagedKV& p, int b) { return ARKE_CHK(b, b, p.B) ? p.lens[b] : 0; }
+__device__ __forceinline__ int table_at(const PagedKV& p, int b, int page) {
+  return ARKE_CHK(b, b, p.B) && ARKE_CHK(page, page, p.max_pages) ? p.table[b * p.ldt + page] : -1;
+}
+
+__device__ __forceinline__ int seq_begin(const PagedKV& p, int b) { return p.cu ? cu_at(p, b) : b * p.uniform; }
 
 // cu_q as the kernels use it: clamped to [0, T], so that no offset of a corrupt table leaves the call's rows
 __device__ __forceinline__ int seq_begin_clamped(const PagedKV& p, int b) {
@@ -44,7 +51,7 @@ __device__ __forceinline__ int find_sequence_warp(const PagedKV& p, int t) {
   while (hi - lo > 0) {
     const int step = (hi - lo + 31) / 32;
     const int at = lo + (lane + 1) * step - 1;   // last entry of this lane's part
-    const bool le = at < hi && p.cu[at] <= t;
+    const bool le = at < hi && cu_at(p, at) <= t;
     const unsigned m = __ballot_sync(0xffffffffu, le);
     const int full = m == 0xffffffffu ? 32 : __ffs(~m) - 1;   // parts that lie at or below t altogether
     lo = lo + full * step;
@@ -60,7 +67,7 @@ __device__ __forceinline__ int find_sequence_warp(const PagedKV& p, int t) {
 __device__ __forceinline__ int find_sequence_lanes(const PagedKV& p, int t) {
   if (p.cu == nullptr) return p.uniform > 0 ? min(t / p.uniform, p.B) : p.B;
   int b = find_sequence_warp(p, __shfl_sync(0xffffffffu, t, 0));
-  while (b < p.B && p.cu[b + 1] <= t) ++b;
+  while (b < p.B && cu_at(p, b + 1) <= t) ++b;
   return b;
 }
 

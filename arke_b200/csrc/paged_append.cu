@@ -52,12 +52,12 @@ __device__ __forceinline__ AppendPlace append_place(const AppendParams& p, int t
   a.row = 0;
   if (b < 0 || b >= p.kv.B) { a.seq = -1; return a; }
   const int s0 = seq_begin(p.kv, b), s1 = seq_begin(p.kv, b + 1);
-  const int64_t pos = (int64_t)p.kv.lens[b] - (s1 - s0) + (t - s0);
-  const int64_t rot = p.positions ? (int64_t)p.positions[t] : pos;
+  const int64_t pos = (int64_t)len_at(p.kv, b) - (s1 - s0) + (t - s0);
+  const int64_t rot = p.positions ? (ARKE_CHK(t, t, p.T) ? (int64_t)p.positions[t] : -1) : pos;
   if (rot >= 0 && rot < p.table_rows) a.rot = rot;
   if (pos >= 0 && pos < (int64_t)p.kv.max_pages * p.kv.page_size) {
     const int pg = (int)(pos / p.kv.page_size);
-    const int id = p.kv.table[b * p.kv.ldt + pg];
+    const int id = table_at(p.kv, b, pg);
     if (id >= 0 && id < p.kv.num_pages) { a.page = id; a.row = (int)(pos - (int64_t)pg * p.kv.page_size); }
   }
   return a;
@@ -92,6 +92,15 @@ __device__ __forceinline__ bool append_chk(const AppendParams& p, const T* dst, 
 #else
 #define ARKE_APPEND_CHK(p, dst, t, h, j, n) (true)
 #endif
+// n elements from x's (t, h, j) on, and half a head further; n angles of row `rot`
+__device__ __forceinline__ bool append_chk_x(const AppendParams& p, int t, int h, int j, int n) {
+  [[maybe_unused]] const long long so = (long long)t * p.ldx + (long long)h * p.D + j;
+  return ARKE_CHK(so, so + (p.D >> 1) + n - 1, span_elems(p.T, (long long)(p.Hq + 2 * p.kv.Hkv) * p.D, p.ldx));
+}
+__device__ __forceinline__ bool append_chk_angle(const AppendParams& p, int64_t rot, int j, int n) {
+  [[maybe_unused]] const long long at = rot * (p.D >> 1) + j;
+  return ARKE_CHK(at, at + n - 1, p.table_rows * (p.D >> 1));
+}
 
 template <typename TT>
 __device__ __forceinline__ void load_table(const TT* src, float (&v)[8]) {
@@ -124,7 +133,7 @@ __global__ void __launch_bounds__(128) paged_append_vec_kernel(const AppendParam
     h[u] = idx / vpu;
     j[u] = (idx - h[u] * vpu) * 8;
     a[u] = b[u] = make_uint4(0, 0, 0, 0);
-    if (h[u] < htot) {
+    if (h[u] < htot && append_chk_x(p, t, h[u], j[u], 8)) {
       const T* src = row + h[u] * p.D + j[u];
       a[u] = __ldcs(reinterpret_cast<const uint4*>(src));
       b[u] = __ldcs(reinterpret_cast<const uint4*>(src + half));
@@ -149,7 +158,7 @@ __global__ void __launch_bounds__(128) paged_append_vec_kernel(const AppendParam
     if (h[u] < p.Hq + p.kv.Hkv) {
       if (have != j[u]) {
         have = j[u];
-        if (at.rot >= 0) {
+        if (at.rot >= 0 && append_chk_angle(p, at.rot, j[u], 8)) {
           load_table<TT>(reinterpret_cast<const TT*>(p.cos) + at.rot * half + j[u], c);
           load_table<TT>(reinterpret_cast<const TT*>(p.sin) + at.rot * half + j[u], s);
         } else {
@@ -197,7 +206,7 @@ __global__ void __launch_bounds__(128) paged_append_scalar_kernel(const AppendPa
   T a = src[0], b = src[half];
   if (h < p.Hq + p.kv.Hkv) {
     float c = __int_as_float(0x7fc00000), s = c;
-    if (at.rot >= 0) {
+    if (at.rot >= 0 && append_chk_angle(p, at.rot, j, 1)) {
       c = to_f32(reinterpret_cast<const TT*>(p.cos)[at.rot * half + j]);
       s = to_f32(reinterpret_cast<const TT*>(p.sin)[at.rot * half + j]);
     }

@@ -36,7 +36,13 @@ struct PagedAttParams {
   float* tile_o[2];           // [2 * split][T * Hq][D]: prefix, sequences
   float* tile_ml[2];          // [2 * split][T * Hq][2]
   int* status;
+  // what the checked build holds every access against: q's first element before its pointer and elements from there on,
+  // rows of the workspace's parts
+  int64_t q_before, q_ext;
+  int64_t part_rows, row_rows, tile_rows[2];
 };
+// n elements of q from offset `at` on
+__device__ __forceinline__ bool q_chk(const PagedAttParams& p, int64_t at, int n) { return ARKE_CHK(at + p.q_before, at + p.q_before + n - 1, p.q_ext); }
 
 // Keys of sequence b behind the shared prefix (0 when there is none), in tiles.
 struct SeqWork {
@@ -48,14 +54,14 @@ __device__ __forceinline__ SeqWork seq_work(const PagedAttParams& p, int b) {
   const int s0 = seq_begin_clamped(p.kv, b), s1 = seq_begin_clamped(p.kv, b + 1);
   w.n = s1 > s0 ? s1 - s0 : 0;
   const int cap = p.kv.max_pages * p.kv.page_size;
-  const int len = p.kv.lens[b];
+  const int len = len_at(p.kv, b);
   w.len = len < 0 ? 0 : len > cap ? cap : len;
   w.tiles = w.len > p.prefix && !seq_in_tiles(p, w.n) ? (w.len - p.prefix + p.tile - 1) / p.tile : 0;
   return w;
 }
 // Entry `page` of sequence b's row of the block table (b = -1: the shared prefix).
 __device__ __forceinline__ int page_of(const PagedAttParams& p, int b, int page) {
-  return p.kv.table[(page < p.shared_pages ? 0 : b) * p.kv.ldt + page];
+  return table_at(p.kv, page < p.shared_pages ? 0 : b, page);
 }
 // Positions that query row `token` of sequence b sees (0: no such sequence).
 __device__ __forceinline__ int seen_by(const PagedAttParams& p, int b, int token) {

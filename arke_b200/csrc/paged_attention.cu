@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(kPagThreads, 2) paged_gqa_kernel(const PagedAt
           for (int i = 0; i < kPagWarps; ++i) {
             if (begin <= s_first[i] && s_first[i] < end) { s_seq[i] = b; s_base[i] = begin; }
           }
-        if (blockIdx.x == 0 && b < p.kv.B) p.sched[2 + b] = begin;
+        if (blockIdx.x == 0 && b < p.kv.B && ARKE_CHK(b, b, p.kv.B)) p.sched[2 + b] = begin;
       }
       __syncthreads();
     }
@@ -323,11 +323,13 @@ __global__ void __launch_bounds__(kPagThreads, 2) paged_gqa_kernel(const PagedAt
       for (int nt = 0; nt < NT; ++nt) {
         const int orow = __shfl_sync(0xffffffffu, my_row, (nt * 8 + (lane >> 2)) & 31);
         const int token = orow / p.Hq;
-        const T* src = reinterpret_cast<const T*>(p.q) + token * p.q_st + (int64_t)(orow - token * p.Hq) * p.q_sh + 2 * (lane & 3);
+        const int64_t at = token * p.q_st + (int64_t)(orow - token * p.Hq) * p.q_sh;
+        const bool ok = orow >= 0 && q_chk(p, at, D);
+        const T* src = reinterpret_cast<const T*>(p.q) + at + 2 * (lane & 3);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          qf[nt][ks][0] = orow >= 0 ? *reinterpret_cast<const uint32_t*>(src + ks * 16) : 0u;
-          qf[nt][ks][1] = orow >= 0 ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + 8) : 0u;
+          qf[nt][ks][0] = ok ? *reinterpret_cast<const uint32_t*>(src + ks * 16) : 0u;
+          qf[nt][ks][1] = ok ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + 8) : 0u;
         }
       }
       float acc[KS][NT][4];
@@ -499,13 +501,14 @@ __global__ void __launch_bounds__(kPagThreads, 2) paged_gqa_kernel(const PagedAt
           if (p.lse && lane < 4)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-              if (orow[e] >= 0) p.lse[orow[e]] = l[nt][e] == 0.f ? -INFINITY : (mx[nt][e] + log2f(l[nt][e])) * 0.6931471805599453f;
+              if (orow[e] >= 0 && ARKE_CHK(orow[e], orow[e], (int64_t)p.kv.T * p.Hq)) p.lse[orow[e]] = l[nt][e] == 0.f ? -INFINITY : (mx[nt][e] + log2f(l[nt][e])) * 0.6931471805599453f;
         } else {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             if (orow[e] < 0) continue;
             const int64_t slot = whole ? orow[e] + (cur.b >= 0 ? (int64_t)p.kv.T * p.Hq : 0)
                                        : (worker * 2 + (starts ? 1 : 0)) * R + nt * 8 + 2 * (lane & 3) + e;
+            if (!ARKE_CHK(slot, slot, whole ? p.row_rows : p.part_rows)) continue;
             float* po = (whole ? p.row_o : p.part_o) + slot * D + (lane >> 2);
 #pragma unroll
             for (int i = 0; i < KS; ++i) {
@@ -540,7 +543,8 @@ __device__ __forceinline__ void join_row(const PagedAttParams& p, int R, int64_t
 #pragma unroll
   for (int i = 0; i < V; ++i) v[i] = 0.f;
   const bool live = b >= 0 && b < p.kv.B;
-  const bool bad = live && (p.kv.lens[b] < 0 || p.kv.lens[b] > p.kv.max_pages * p.kv.page_size);
+  const int len = live ? len_at(p.kv, b) : 0;
+  const bool bad = len < 0 || len > p.kv.max_pages * p.kv.page_size;
   SeqWork sw{0, 0, 0};
   int rr = 0;
   // the four kinds of pieces: tensor-core parts of the prefix and of the sequence, streamed ones of both
@@ -585,7 +589,7 @@ __device__ __forceinline__ void join_row(const PagedAttParams& p, int R, int64_t
     }
     if (sw.tiles > 0) {
       const int nrb = row_blocks(p, sw.n, R), rb = rr / R;
-      const int64_t s0 = p.sched[2 + b] + ((int64_t)h * nrb + rb) * sw.tiles;
+      const int64_t s0 = (ARKE_CHK(b, b, p.kv.B) ? p.sched[2 + b] : 0) + ((int64_t)h * nrb + rb) * sw.tiles;
       lo[1] = shares.warp_at(s0);
       count[3] = (int)(shares.warp_at(s0 + sw.tiles - 1) - lo[1]) + 1;
       r[1] = rr - rb * R;
@@ -607,7 +611,7 @@ __device__ __forceinline__ void join_row(const PagedAttParams& p, int R, int64_t
           unit_steps(kind ? seq_unit_keys(p, sw, rr / kTileRows * kTileRows, kTileRows) : prefix_unit_keys(p), kind ? p.seq_split : p.pre_split,
                      s >> two, j0, j1);
           if (two && (s & 1)) ++j0;                     // the second half has the odd steps
-          if (j0 < j1) po = (kind ? p.tile_o[1] : p.tile_o[0]) + (s * all + row) * D;
+          if (j0 < j1 && ARKE_CHK(s * all + row, s * all + row, p.tile_rows[kind])) po = (kind ? p.tile_o[1] : p.tile_o[0]) + (s * all + row) * D;
           pm = (kind ? p.tile_ml[1] : p.tile_ml[0]) + (s * all + row) * 2;
         } else {
           i -= count[0] + count[1];
@@ -615,7 +619,7 @@ __device__ __forceinline__ void join_row(const PagedAttParams& p, int R, int64_t
           const int64_t from = u ? lo[1] : lo[0], c = from + i - (u ? count[2] : 0);
           const bool one = u ? whole[1] : whole[0];
           const int64_t slot = one ? row + u * all : (c * 2 + (c == from ? 1 : 0)) * R + (u ? r[1] : r[0]);
-          po = (one ? p.row_o : p.part_o) + slot * D;
+          if (ARKE_CHK(slot, slot, one ? p.row_rows : p.part_rows)) po = (one ? p.row_o : p.part_o) + slot * D;
           pm = (one ? p.row_ml : p.part_ml) + slot * 2;
         }
         if (po) q = *reinterpret_cast<const float2*>(pm);
@@ -718,6 +722,7 @@ static bool split_prefix(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t 
 }
 struct PagLayout {
   size_t sched, part_o, part_ml, row_o, row_ml, tile_o[2], tile_ml[2], total;
+  int64_t part_rows, row_rows, tile_rows[2];
 };
 static PagLayout pag_layout(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t prefix, int grid) {
   auto up = [](size_t v) { return (v + 255) / 256 * 256; };
@@ -736,7 +741,10 @@ static PagLayout pag_layout(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64
   for (int i = 0; i < 2; ++i) {
     w.tile_o[i] = at;  at += up(sizeof(float) * (size_t)tile[i] * (size_t)D);
     w.tile_ml[i] = at; at += up(sizeof(float) * (size_t)tile[i] * 2);
+    w.tile_rows[i] = tile[i];
   }
+  w.part_rows = (int64_t)slots;
+  w.row_rows = 2 * (int64_t)rows;
   w.total = at;
   return w;
 }
@@ -844,6 +852,12 @@ extern "C" int arke_b200_paged_gqa_fwd(const void* q, int64_t q_stride_token, in
   p.row_o = reinterpret_cast<float*>(ws + w.row_o);
   p.row_ml = reinterpret_cast<float*>(ws + w.row_ml);
   p.grid = grid;
+  const int64_t far_t = (T - 1) * q_stride_token, far_h = (Hq - 1) * q_stride_head;
+  p.q_before = -((far_t < 0 ? far_t : 0) + (far_h < 0 ? far_h : 0));
+  p.q_ext = p.q_before + (far_t > 0 ? far_t : 0) + (far_h > 0 ? far_h : 0) + D;
+  p.part_rows = w.part_rows;
+  p.row_rows = w.row_rows;
+  for (int i = 0; i < 2; ++i) p.tile_rows[i] = w.tile_rows[i];
   p.status = kernel_status_ptr();
   if (!p.status) return ARKE_ERR_CUDA;
   cudaStream_t st = (cudaStream_t)stream;

@@ -373,10 +373,12 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     // ---- this thread's row of Q, in the layout the tensor core reads (128-byte rows, 16-byte chunks swizzled)
     if (n_t > 0 && !geo.q_tma) {
       uint8_t* dst = smem + SM::kQOff + t * SM::kTileBytes + row_in_tile * 128;
-      const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.q) + token * p.q_st + head * p.q_sh);
+      const int64_t at = token * p.q_st + head * p.q_sh;
+      const bool copy = row_ok && q_chk(p, at, D);
+      const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.q) + at);
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) {
-        const uint4 v = row_ok ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+        const uint4 v = copy ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
         *reinterpret_cast<uint4*>(dst + (i >> 3) * SM::kChunkBytes + (((i & 7) ^ (row_in_tile & 7)) << 4)) = v;
       }
       fence_async_smem();
@@ -501,10 +503,11 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       tc_fence_after();
       const int64_t all = (int64_t)p.kv.T * p.Hq;
       const int orow = row_ok ? token * p.Hq + head : -1;
-      const bool write = orow >= 0 && ARKE_CHK((int64_t)orow * D, (int64_t)orow * D + D - 1, all * D);
-      const unsigned live = __ballot_sync(0xffffffffu, write);
       const bool final_here = b >= 0 && !dual && p.seq_split == 1 && p.prefix == 0;
       const int slot = dual ? 2 * part + t : part;
+      [[maybe_unused]] const int64_t out_row = final_here ? orow : slot * all + orow, out_rows = final_here ? all : p.tile_rows[b >= 0];
+      const bool write = orow >= 0 && ARKE_CHK(orow, orow, all) && ARKE_CHK(out_row, out_row, out_rows);
+      const unsigned live = __ballot_sync(0xffffffffu, write);
       // a missing page, or nothing seen (NaN scores leave a sum): O is not what tensor memory holds
       const bool broken = *bad_flag != 0, none = broken || m_used == -INFINITY;
       const float fill = broken || l != 0.f ? __uint_as_float(0x7fc00000u) : 0.f;

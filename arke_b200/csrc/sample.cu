@@ -685,6 +685,7 @@ __global__ void __launch_bounds__(kSmpThreads, FILTERS ? 2 : 3) sample_kernel(co
   r.limb = __clz(p.slice - 1);                           // slice <= 2^(32 - limb); 15 bits at V = 2^20
   const T* src = reinterpret_cast<const T*>(p.x) + (int64_t)row * p.ld + r.first;
   r.src = p.staged ? stage : src;
+  if (!ARKE_CHK(row, row, p.B)) return;                  // every setting and output of the row; the same for the whole cluster
   const float t = p.t_row ? p.t_row[row] : p.t, pp = p.p_row ? p.p_row[row] : p.p;
   const float r_min_p = fminf(p.m_row ? p.m_row[row] : p.m, 1.f);
   const int k = p.k_row ? p.k_row[row] : p.k;
