@@ -13,8 +13,11 @@ fallback — the op body always runs the sm_100a kernel.
     q      = torch.ops.arke.qkv_rope_paged_append(qkv, cos, sin, k_cache, v_cache, table, kv_lens, cu_q, Hq)
     o, lse = torch.ops.arke.paged_gqa_fwd(q, k_cache, v_cache, table, kv_lens, cu_q, prefix)
     tok    = torch.ops.arke.sample_tokens(logits, u, 0.8, 50, 0.95, 0.0)
+    tok, lp = torch.ops.arke.sample_tokens_logprob(logits, u, temperature_rows=t, top_p_rows=p)
 """
 from __future__ import annotations
+
+from typing import Optional
 
 import torch
 
@@ -24,7 +27,7 @@ _REGISTERED = False
 def register_ops() -> bool:
     """Registers ``arke::rmsnorm``, ``arke::rmsnorm_quant``, ``arke::quantize_per_token``, ``arke::w8a8_gemm``, ``arke::swiglu_fp8``,
     ``arke::gqa_fwd``, ``arke::rope``, ``arke::qkv_rope_split``, ``arke::fused_linear_ce``, ``arke::qkv_rope_paged_append``,
-    ``arke::paged_gqa_fwd`` and ``arke::sample_tokens``; returns True when (already) registered."""
+    ``arke::paged_gqa_fwd``, ``arke::sample_tokens`` and ``arke::sample_tokens_logprob``; returns True when (already) registered."""
     global _REGISTERED
     if _REGISTERED:
         return True
@@ -107,29 +110,51 @@ def register_ops() -> bool:
 
     @torch.library.custom_op("arke::qkv_rope_paged_append", mutates_args=("k_cache", "v_cache"))
     def qkv_rope_paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
-                              block_table: torch.Tensor, kv_lens: torch.Tensor, cu_q: torch.Tensor, Hq: int) -> torch.Tensor:
-        return ops.qkv_rope_paged_append(qkv, cos, sin, k_cache, v_cache, block_table, kv_lens, Hq, cu_q=cu_q)
+                              block_table: torch.Tensor, kv_lens: torch.Tensor, cu_q: Optional[torch.Tensor], Hq: int,
+                              positions: Optional[torch.Tensor] = None) -> torch.Tensor:
+        return ops.qkv_rope_paged_append(qkv, cos, sin, k_cache, v_cache, block_table, kv_lens, Hq, cu_q=cu_q, positions=positions)
 
     @qkv_rope_paged_append.register_fake
-    def _(qkv, cos, sin, k_cache, v_cache, block_table, kv_lens, cu_q, Hq):
+    def _(qkv, cos, sin, k_cache, v_cache, block_table, kv_lens, cu_q, Hq, positions=None):
         return qkv.new_empty((qkv.shape[0], Hq, k_cache.shape[3]))
 
     @torch.library.custom_op("arke::paged_gqa_fwd", mutates_args=())
     def paged_gqa_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor,
-                      cu_q: torch.Tensor, shared_prefix: int) -> tuple[torch.Tensor, torch.Tensor]:
-        return ops.paged_gqa_fwd(q, k_cache, v_cache, block_table, kv_lens, cu_q=cu_q, shared_prefix=shared_prefix)
+                      cu_q: Optional[torch.Tensor], shared_prefix: int, causal: bool = True, softmax_scale: Optional[float] = None,
+                      max_new: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
+        return ops.paged_gqa_fwd(q, k_cache, v_cache, block_table, kv_lens, cu_q=cu_q, shared_prefix=shared_prefix, causal=causal,
+                                 softmax_scale=softmax_scale, max_new=max_new)
 
     @paged_gqa_fwd.register_fake
-    def _(q, k_cache, v_cache, block_table, kv_lens, cu_q, shared_prefix):
+    def _(q, k_cache, v_cache, block_table, kv_lens, cu_q, shared_prefix, causal=True, softmax_scale=None, max_new=0):
         return torch.empty_like(q, memory_format=torch.contiguous_format), q.new_empty(q.shape[:-1], dtype=torch.float32)
 
+    # a setting is the number, or the vector of one value per row where it is given
+    def either(rows, number):
+        return number if rows is None else rows
+
     @torch.library.custom_op("arke::sample_tokens", mutates_args=())
-    def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: float, top_k: int, top_p: float, min_p: float) -> torch.Tensor:
-        return ops.sample_tokens(logits, u, temperature, top_k, top_p, min_p)
+    def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+                      min_p: float = 0.0, temperature_rows: Optional[torch.Tensor] = None, top_k_rows: Optional[torch.Tensor] = None,
+                      top_p_rows: Optional[torch.Tensor] = None, min_p_rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+        return ops.sample_tokens(logits, u, either(temperature_rows, temperature), either(top_k_rows, top_k), either(top_p_rows, top_p),
+                                 either(min_p_rows, min_p))
 
     @sample_tokens.register_fake
-    def _(logits, u, temperature, top_k, top_p, min_p):
+    def _(logits, u, *args, **kwargs):
         return logits.new_empty((logits.shape[0],), dtype=torch.int64)
+
+    @torch.library.custom_op("arke::sample_tokens_logprob", mutates_args=())
+    def sample_tokens_logprob(logits: torch.Tensor, u: torch.Tensor, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+                              min_p: float = 0.0, temperature_rows: Optional[torch.Tensor] = None,
+                              top_k_rows: Optional[torch.Tensor] = None, top_p_rows: Optional[torch.Tensor] = None,
+                              min_p_rows: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+        return ops.sample_tokens(logits, u, either(temperature_rows, temperature), either(top_k_rows, top_k), either(top_p_rows, top_p),
+                                 either(min_p_rows, min_p), return_logprob=True)
+
+    @sample_tokens_logprob.register_fake
+    def _(logits, u, *args, **kwargs):
+        return logits.new_empty((logits.shape[0],), dtype=torch.int64), logits.new_empty((logits.shape[0],), dtype=torch.float32)
 
     _REGISTERED = True
     return True
