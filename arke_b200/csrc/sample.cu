@@ -169,12 +169,15 @@ struct SmpShared {
   int where;                                // that warp, or -1: another CTA's
   alignas(16) uint32_t bin[4][kSmpBins];    // a bin's sum in words of Row::limb bits and what the additions carry
   uint32_t count;                           // values of one bin in this CTA
-  u64 list[kSmpThreads];                    // those of the cluster: weights, keys
-  uint32_t list_key[kSmpThreads];
+  // The values of one bin, once the histogram has been read: this CTA's in bin[0] and bin[1], the cluster's in bin[2].
+  __device__ __forceinline__ uint32_t* near_key() { return bin[0]; }
+  __device__ __forceinline__ u64* near_weight() { return reinterpret_cast<u64*>(bin[1]); }
+  __device__ __forceinline__ u64* list() { return reinterpret_cast<u64*>(bin[2]); }
+  __device__ __forceinline__ uint32_t* list_key() { return bin[2] + 2 * kSmpThreads; }
 };
-// 64-bit weights are queued in bin[1], and the CTAs' structures lie at multiples of 128 bytes
-static_assert(offsetof(SmpShared, bin) % 16 == 0 && offsetof(SmpShared, list) % 8 == 0 && offsetof(SmpShared, target) % 16 == 0);
-static_assert(kSmpThreads * sizeof(u64) <= sizeof(uint32_t) * kSmpBins && kSmpWarps * 160 <= 4 * kSmpBins);
+// the structure lies at a multiple of 128 bytes; 64-bit weights in the bins
+static_assert(offsetof(SmpShared, bin) % 16 == 0 && offsetof(SmpShared, target) % 16 == 0 && kSmpBins % 4 == 0);
+static_assert(3 * kSmpThreads <= kSmpBins && kSmpWarps * 160 <= 4 * kSmpBins);
 
 template <typename T, int CS>
 struct Row {
@@ -234,8 +237,7 @@ struct Row {
   }
   // in the histogram's steps
   __device__ __forceinline__ u64 binned(float f) const {
-    const double y = scaled(f);
-    return fine ? __double2ull_rn(y * kSmpFine) : (u64)__double_as_longlong(y + 4503599627370496.0) & 0xfffffffffffffull;
+    return __double2ull_rn(scaled(f) * (fine ? kSmpFine : 1.0));
   }
   // coarse bin of a value, 0 = the highest: 1/64 of a logit each, the last takes the rest (and NaN)
   __device__ __forceinline__ int coarse(float f) const {
@@ -482,11 +484,9 @@ __device__ __forceinline__ Sum<WEIGHT> found_rest(const SmpShared& s) {
 }
 
 template <bool WEIGHT>
-__device__ __forceinline__ void clear_bins(SmpShared& s) {
-  for (int j = threadIdx.x; j < kSmpBins; j += kSmpThreads) {
-    s.bin[0][j] = 0;
-    if constexpr (WEIGHT) s.bin[1][j] = s.bin[2][j] = s.bin[3][j] = 0;
-  }
+__device__ __forceinline__ void clear_bins(SmpShared& s, bool fine) {
+  const int words = !WEIGHT ? 1 : fine ? 4 : 3;
+  for (int j = threadIdx.x; j < words * kSmpBins / 4; j += kSmpThreads) reinterpret_cast<uint4*>(s.bin)[j] = make_uint4(0, 0, 0, 0);
   __syncthreads();
 }
 // Adds without reading back: an atomic whose result nobody waits for costs a slot, not a round trip.
@@ -512,7 +512,7 @@ template <bool WEIGHT, typename T, int CS>
 __device__ __forceinline__ void find_threshold(Row<T, CS>& r, const Goal<WEIGHT>& goal, float least, uint32_t& K, Sum<WEIGHT>& rest, u64& equals) {
   SmpShared& s = *r.s;
   const int tid = threadIdx.x;
-  clear_bins<WEIGHT>(s);
+  clear_bins<WEIGHT>(s, r.fine);
 #pragma unroll 4
   for (int i = tid; i < r.n; i += kSmpThreads) {
     const float f = r.at(i);
@@ -530,8 +530,8 @@ __device__ __forceinline__ void find_threshold(Row<T, CS>& r, const Goal<WEIGHT>
   if (klo < khi) {
     // A bin of few values is resolved in one step: every CTA gets all of them and adds up, for each of its own, what
     // lies above it and what equals it.
-    uint32_t* const near_key = s.bin[0];                  // this CTA's values of the bin
-    u64* const near_weight = reinterpret_cast<u64*>(s.bin[1]);
+    uint32_t* const near_key = s.near_key();
+    u64* const near_weight = s.near_weight();
     if (tid == 0) s.count = 0;
     __syncthreads();
     for (int i0 = tid; i0 < r.n; i0 += 4 * kSmpThreads) {
@@ -574,20 +574,20 @@ __device__ __forceinline__ void find_threshold(Row<T, CS>& r, const Goal<WEIGHT>
         const u64 w = near_weight[tid];
 #pragma unroll
         for (uint32_t c = 0; c < CS; ++c) {
-          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_cluster(smem_u32(&s.list_key[first + tid]), c)), "r"(k) : "memory");
-          st_cluster_u64(mapa_cluster(smem_u32(&s.list[first + tid]), c), w);
+          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_cluster(smem_u32(&s.list_key()[first + tid]), c)), "r"(k) : "memory");
+          st_cluster_u64(mapa_cluster(smem_u32(&s.list()[first + tid]), c), w);
         }
       }
       const Sum<WEIGHT> left = found_rest<WEIGHT>(s);
       cluster_sync_all();
       // eight lanes to each of this CTA's own values
       for (uint32_t e0 = 0; e0 < own; e0 += kSmpThreads / 8) {
-        const uint32_t e = e0 + tid / 8, k = s.list_key[first + min(e, own - 1)];
+        const uint32_t e = e0 + tid / 8, k = s.list_key()[first + min(e, own - 1)];
         Sum<WEIGHT> more = 0, same = 0;
 #pragma unroll 4
         for (uint32_t i = tid & 7; i < n; i += 8) {
-          const u64 w = s.list[i];
-          const uint32_t ki = s.list_key[i];
+          const u64 w = s.list()[i];
+          const uint32_t ki = s.list_key()[i];
           more += ki > k ? w : 0;
           same += ki == k ? w : 0;
         }
@@ -617,7 +617,7 @@ __device__ __forceinline__ void find_threshold(Row<T, CS>& r, const Goal<WEIGHT>
     const uint32_t span = khi - klo;
     const int bits = 32 - __clz(span), shift = bits > 11 ? bits - 11 : 0;
     const Goal<WEIGHT> left{found_rest<WEIGHT>(s), 0.f, 0};
-    clear_bins<WEIGHT>(s);
+    clear_bins<WEIGHT>(s, r.fine);
 #pragma unroll 4
     for (int i = tid; i < r.n; i += kSmpThreads) {
       const float f = r.at(i);
@@ -642,7 +642,7 @@ __device__ __forceinline__ void find_threshold(Row<T, CS>& r, const Goal<WEIGHT>
 
 // the least n with n w >= rest, for a rest of up to 2^20 w
 __device__ __forceinline__ u64 how_many(u128 rest, u64 w) {
-  if (w == 0) return 1;
+  if (w == 0 || rest <= w) return 1;
   u64 n = (u64)(real(rest) / (double)w);
   while (n > 1 && (u128)(n - 1) * w >= rest) --n;
   while ((u128)n * w < rest) ++n;
@@ -658,7 +658,7 @@ __device__ __forceinline__ void find_top_p(Row<T, CS>& r, float p, float least, 
   for (r.fine = false;; r.fine = true) {
     u128 rest;
     u64 unused;
-    find_threshold<true>(r, Goal<true>{0, p, (u128)surplus * r.binned(least)}, least, K, rest, unused);
+    find_threshold<true>(r, Goal<true>{0, p, surplus ? (u128)surplus * r.binned(least) : 0}, least, K, rest, unused);
     const float f = r.value(K);
     const u64 w = r.binned(f), margin = (u64)V + 2;
     allowed = how_many(rest, w);
@@ -679,6 +679,7 @@ __global__ void __launch_bounds__(kSmpThreads, FILTERS ? 2 : 3) sample_kernel(co
   Row<T, CS> r;
   r.rank = CS == 1 ? 0 : cluster_ctarank();
   r.s = &s;
+  r.fine = false;
   const int row = blockIdx.x / CS;
   r.first = (int)r.rank * p.slice;
   r.n = max(0, min(p.slice, p.V - r.first));
@@ -761,13 +762,13 @@ __global__ void __launch_bounds__(kSmpThreads, FILTERS ? 2 : 3) sample_kernel(co
   __syncthreads();
 
   const float u = u_row > 0.f ? u_row : 0.f;
+  // min-p as a limit of the logits: the least float that is not below max + T ln(min_p), less what the exponential of
+  // 64 bits rounds up to min_p (2^-54, for min_p = 1 at temperatures that leave nothing of the differences)
+  const float floor = r_min_p > 0.f && r.top < INFINITY
+                          ? __double2float_ru((double)r.top + (double)t * (log((double)r_min_p) - 5.551115123125783e-17)) : -INFINITY;
   if (!FILTERS || (!(k > 0 && k < p.V) && !(pp < 1.f))) {
-    // min-p as a limit of the logits: the least float that is not below max + T ln(min_p), less what the exponential
-    // of 64 bits rounds up to min_p (2^-54, for min_p = 1 at temperatures that leave nothing of the differences)
-    const double limit = (double)r.top + (double)t * (log((double)fmaxf(r_min_p, 0.f)) - 5.551115123125783e-17);
     const float cut = fmaxf((float)((double)r.top - 33.3 * (double)t), -3.402823466e38f);      // 2^-48 of the largest
-    const float least = fmaxf(r_min_p > 0.f && r.top < INFINITY ? __double2float_ru(limit) : -INFINITY, cut);
-    if (estimate(r, p, row, least, u)) return;
+    if (estimate(r, p, row, fmaxf(floor, cut), u)) return;
   }
 
   // ---- the value that still stays in, and how many of its equals
@@ -788,21 +789,17 @@ __global__ void __launch_bounds__(kSmpThreads, FILTERS ? 2 : 3) sample_kernel(co
   }
 
   // ---- sums of what stays in, in the order of the vocabulary: a contiguous part for each warp
-  const double y_min = (double)fmaxf(r_min_p, 0.f) * kSmpOne;
+  r.cut = fmaxf(r.cut, floor);
   const bool filtered = FILTERS && allowed != ~0ull;
   const float fk = filtered ? r.value(K) : -INFINITY;    // above it all stay in, of its equals the first `allowed`
-  const u128 w_eq = filtered && r.scaled(fk) >= y_min ? r.weight(fk) : 0;
+  const u128 w_eq = filtered ? r.weight(fk) : 0;
   const int part = (r.n + kSmpWarps * 32 - 1) / (kSmpWarps * 32) * 32;
   const int i0 = min(warp * part, r.n), i1 = min(i0 + part, r.n);
-  auto add = [&](float f, u64& hi, u64& lo) {
-    const double y = r.scaled(f);
-    r.add_raw(y >= y_min ? y : 0.0, hi, lo);
-  };
   u64 hi = 0, lo = 0;
   uint32_t eq = 0;
   if (!filtered) {
 #pragma unroll 8
-    for (int i = i0 + lane; i < i1; i += 32) add(r.at(i), hi, lo);
+    for (int i = i0 + lane; i < i1; i += 32) r.add_raw(r.scaled(r.at(i)), hi, lo);
     const u64 added = i1 > i0 + lane ? (i1 - i0 - lane + 31) / 32 : 0;
     hi -= added * r.kHi;
     lo -= added * r.kLo;
@@ -829,14 +826,14 @@ __global__ void __launch_bounds__(kSmpThreads, FILTERS ? 2 : 3) sample_kernel(co
       __syncwarp();
       while (n >= 32) {                                  // from the end, so that nothing has to move
         n -= 32;
-        add(queue[n + lane], hi, lo);
+        r.add_raw(r.scaled(queue[n + lane]), hi, lo);
         hi -= r.kHi;
         lo -= r.kLo;
       }
       __syncwarp();
     }
     if (lane < n) {
-      add(queue[lane], hi, lo);
+      r.add_raw(r.scaled(queue[lane]), hi, lo);
       hi -= r.kHi;
       lo -= r.kLo;
     }
@@ -889,11 +886,10 @@ __global__ void __launch_bounds__(kSmpThreads, FILTERS ? 2 : 3) sample_kernel(co
     // The first token that is kept and whose weight is not zero in 64 bits: below e^-745.13 it is.  Its index as the
     // maximum of the complement.
     u64 at = 0;
-    const double ln_min = r_min_p > 0.f ? log((double)r_min_p) : -INFINITY;
     for (int i = tid; i < r.n; i += kSmpThreads) {
       const float f = r.at(i);
       const double e = f == r.top ? 0.0 : ((double)f - (double)r.top) * r.inv_t;
-      if (f >= fk && e > -745.13 && (f >= r.cut ? r.scaled(f) >= y_min : e >= ln_min)) { at = (uint32_t)~(uint32_t)(r.first + i); break; }
+      if (f >= fk && f >= floor && e > -745.13) { at = (uint32_t)~(uint32_t)(r.first + i); break; }
     }
     at = warp_max(at);
     __syncthreads();
@@ -919,7 +915,7 @@ __global__ void __launch_bounds__(kSmpThreads, FILTERS ? 2 : 3) sample_kernel(co
     const float f = r.at(i);
     if (f == fk) ++eq;
     if (f > fk) {
-      add(f, hi, lo);
+      r.add_raw(r.scaled(f), hi, lo);
       hi -= r.kHi;
       lo -= r.kLo;
     }
@@ -932,7 +928,7 @@ __global__ void __launch_bounds__(kSmpThreads, FILTERS ? 2 : 3) sample_kernel(co
       const float f = r.at(i);
       if (f == fk) ++mine.n;
       if (f > fk) {
-        add(f, mine.hi, mine.lo);
+        r.add_raw(r.scaled(f), mine.hi, mine.lo);
         mine.hi -= r.kHi;
         mine.lo -= r.kLo;
       }
