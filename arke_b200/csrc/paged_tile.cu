@@ -617,7 +617,8 @@ void plan_paged_tiles(PagedAttParams& p, const arke_b200_paged_kv* d, int sms) {
   // (512 tokens over 4096 positions beside 511 empty slots, 32 / 8 heads, D = 128: 606 us unknown, 76 us told, 58 us
   // without the slots).  Taking T for granted would put a launch of idle tiles in front of every decode batch.
   p.seq_tile = !p.kv.cu ? (int64_t)p.kv.uniform * p.G > kFewRows
-               : p.kv.max_new ? (int64_t)p.kv.max_new * p.G > kFewRows : (int64_t)(p.kv.T - p.kv.B + 1) * p.G > kTileRows;
+               : p.kv.max_new ? (int64_t)(p.kv.max_new < p.kv.T ? p.kv.max_new : p.kv.T) * p.G > kFewRows
+                              : (int64_t)(p.kv.T - p.kv.B + 1) * p.G > kTileRows;
   const int64_t G = p.G;
   if (p.pre_tile) {
     const int64_t units = tile_units(p.kv.T, p.kv.B, G, p.kv.Hkv, true);

@@ -40,6 +40,7 @@ PADDED = [  # new tokens of each slot, lengths, heads, head_dim, page
     ([0] * 20 + [70] + [0] * 60 + [1, 1, 3] + [0] * 50, [5] * 20 + [70] + [0] * 60 + [90, 31, 3] + [64] * 50, 4, 4, 128, 32),
     ([64] + [0] * 64, [500] + [0] * 64, 8, 1, 64, 8),
     ([0] * 700, [9] * 700, 4, 2, 64, 16),                                                  # nobody has a token
+    ([0] * 9 + [3, 1], [20] * 9 + [300, 2], 8, 2, 64, 16),                                 # fewer rows than a tile wants
 ]
 
 
