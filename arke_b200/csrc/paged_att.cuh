@@ -59,6 +59,18 @@ __device__ __forceinline__ SeqWork seq_work(const PagedAttParams& p, int b) {
   w.tiles = w.len > p.prefix && !seq_in_tiles(p, w.n) ? (w.len - p.prefix + p.tile - 1) / p.tile : 0;
   return w;
 }
+// Where the data of a shared prefix ends, for a whole warp: with its longest sequence at the latest (of those with a token
+// and a length within its range).  What lies behind that nobody has, and it may hold anything; it is read as if it were
+// not there, while units and their steps go by the whole prefix, so that nothing waits for the lengths.
+__device__ __forceinline__ int prefix_data_end(const PagedAttParams& p) {
+  const int cap = p.kv.max_pages * p.kv.page_size;
+  int longest = 0;
+  for (int b = threadIdx.x & 31; b < p.kv.B; b += 32) {
+    const int len = len_at(p.kv, b);
+    if (len <= cap && seq_begin_clamped(p.kv, b + 1) > seq_begin_clamped(p.kv, b)) longest = max(longest, len);
+  }
+  return min(__reduce_max_sync(0xffffffffu, longest), p.prefix);
+}
 // Entry `page` of sequence b's row of the block table (b = -1: the shared prefix).
 __device__ __forceinline__ int page_of(const PagedAttParams& p, int b, int page) {
   return table_at(p.kv, page < p.shared_pages ? 0 : b, page);

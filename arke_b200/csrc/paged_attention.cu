@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(kPagThreads, 2) paged_gqa_kernel(const PagedAt
       cur.tiles = pre_tiles;
       cur.nrb = pre_rb;
       cur.n = tokens;
-      cur.len = p.prefix;
+      cur.len = prefix_data_end(p);
       within = pos0;
     } else {
       cur.open(p, s_seq[warp], R);

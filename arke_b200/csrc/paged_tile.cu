@@ -10,8 +10,8 @@
 //            page), a lane of the loading warp each (one warp for K, one for V: with one for both, pages of 16 ran at
 //            the pace of its instructions, 159 instead of 134 us for the chunk below); pages the sequence does not
 //            have are loaded out of bounds, which fills zeros;
-//   V        rows of the last page behind the sequence's end hold whatever memory held: 0 * NaN would reach O, so
-//            they are zeroed in shared memory before the product (first and last tile only);
+//   V        rows behind the sequence's end in its last page hold whatever memory held: 0 * NaN would reach O, so they
+//            are zeroed in shared memory before the product (the first tile, and the one in which the data ends);
 //   split    a unit's keys are shared out over `split` CTAs, and the (m, l, O) partials meet in the join kernel;
 //   dual     a unit of at most 128 rows has one query tile, whose steps the two pipelines take in turn.
 //
@@ -164,7 +164,6 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     }
   }
   const bool fix_first = j0 * kTileKeys < keys.first;    // V rows that are not this unit's
-  const bool fix_last = (j0 + steps) * kTileKeys > keys.data_end;
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SM::kBarOff);
@@ -177,7 +176,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   uint64_t* p_ready = bars + 12;    // [2] per query tile
   uint64_t* pv_done = bars + 14;    // [2] per query tile
   uint64_t* p_half = bars + 16;     // [2] per query tile: first 64 keys of P are in tensor memory
-  uint64_t* v_fix = bars + 18;      // [2] V rows outside the unit's keys are zero: in the first tile, in the last
+  uint64_t* v_fix = bars + 18;      // [2] V rows in front of the unit's keys are zero; V of the tile in which the data ends has arrived
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SM::kMiscOff);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + SM::kMiscOff + 4);
   volatile int* bad_flag = reinterpret_cast<volatile int*>(smem + SM::kMiscOff + 8);
@@ -209,14 +208,14 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  // Zeroes the V rows of step j outside [first, data_end).  Only for a warp that knows the stage's current phase.
-  auto repair = [&](int j, uint64_t* done) -> bool {
-    const bool got = tile_wait(&v_full[j & 1], (j >> 1) & 1, abort_flag);
+  // Zeroes the V rows of step j outside [first, data_end), which `full` says are there, and reports that to `done`.
+  auto repair = [&](int j, int data_end, uint64_t* full, uint64_t* done) -> bool {
+    const bool got = tile_wait(full, 0, abort_flag);
     if (!__all_sync(0xffffffffu, got)) return false;
     const int k0 = (j0 + j) * kTileKeys;
     uint8_t* v = smem + SM::kVOff + (j & 1) * SM::kTileBytes;
     for (int r = lane; r < kTileKeys; r += 32) {
-      if (k0 + r >= keys.first && k0 + r < keys.data_end) continue;
+      if (k0 + r >= keys.first && k0 + r < data_end) continue;
 #pragma unroll
       for (int c = 0; c < SM::kChunks; ++c)
 #pragma unroll
@@ -244,9 +243,12 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     uint64_t* full = is_k ? k_full : v_full;
     uint64_t* empty = is_k ? k_empty : v_empty;
     uint8_t* dst = smem + (is_k ? SM::kKOff : SM::kVOff) + lane * geo.box_rows * 128;
+    const int data_end = b < 0 ? prefix_data_end(p) : keys.data_end;
+    // the step inside which the data ends, -1 where none does
+    const int fix_step = data_end % kTileKeys != 0 && data_end / kTileKeys >= j0 && data_end / kTileKeys < j1 ? data_end / kTileKeys - j0 : -1;
     auto lookup = [&](int step) -> int {                 // physical page, num_pages (out of bounds) where there is none
       const int key = (j0 + step) * kTileKeys + lane * geo.box_rows;
-      if (lane >= boxes || step >= steps || key >= keys.data_end || key + geo.box_rows <= keys.first) return p.kv.num_pages;
+      if (lane >= boxes || step >= steps || key >= data_end || key + geo.box_rows <= keys.first) return p.kv.num_pages;
       const int id = page_of(p, b, key / p.kv.page_size);
       if (id >= 0 && id < p.kv.num_pages) return id;
       *bad_flag = 1;
@@ -267,19 +269,21 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       const int next = lookup(j + 1);
       ok = tile_wait(&empty[s], ((j >> 1) & 1) ^ 1, abort_flag);
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-      if (lane == 0) mbar_arrive_expect_tx(&full[s], SM::kTileBytes);
+      // V of that step arrives at a barrier of its own, and the stage is full when its rows behind the end are zero
+      const bool fix = !is_k && j == fix_step;
+      uint64_t* arrived = fix ? &v_fix[1] : &full[s];
+      if (lane == 0) mbar_arrive_expect_tx(arrived, SM::kTileBytes);
       __syncwarp();
       if (lane < boxes) {
         const int row = ((j0 + j) * kTileKeys + lane * geo.box_rows) % p.kv.page_size;
 #pragma unroll
         for (int c = 0; c < SM::kChunks; ++c)
-          tma_load_4d(dst + s * SM::kTileBytes + c * SM::kChunkBytes, map, &full[s], c * 64, pick(0, row, page), pick(1, row, page),
+          tma_load_4d(dst + s * SM::kTileBytes + c * SM::kChunkBytes, map, arrived, c * 64, pick(0, row, page), pick(1, row, page),
                       pick(2, row, page));
       }
       page = next;
+      if (fix && !repair(j, data_end, arrived, &full[s])) { ok = false; break; }
     }
-    // the last tile's V: this warp armed its stage last, so its phase is the one to wait for
-    if (ok && !is_k && fix_last) ok = repair(steps - 1, &v_fix[1]);
     if (!ok && lane == 0) tile_abort(p.status, abort_flag, KSTAT_TIMEOUT_PRODUCER);
    } else if (warp == 9) {
     // =============================== MMA issuer ===============================
@@ -314,7 +318,6 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         const int st = step & 1;
         if (!tile_wait(&p_half[t], i & 1, abort_flag) || !tile_wait(&v_full[st], (step >> 1) & 1, abort_flag)) return false;
         if (step == 0 && fix_first && !tile_wait(&v_fix[0], 0, abort_flag)) return false;
-        if (step == steps - 1 && fix_last && !tile_wait(&v_fix[1], 0, abort_flag)) return false;
         tc_fence_after();
         const uint32_t va = v_lo0 + st * kTileLo;
         const uint32_t d = tmem_base + O_COL0 + t * D;
@@ -356,7 +359,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     }
    } else if (warp == 10 && fix_first) {
     // the first tile's V: stage 0 cannot move on before this is done
-    if (!repair(0, &v_fix[0]) && lane == 0) tile_abort(p.status, abort_flag, KSTAT_TIMEOUT_PRODUCER);
+    if (!repair(0, keys.data_end, &v_full[0], &v_fix[0]) && lane == 0) tile_abort(p.status, abort_flag, KSTAT_TIMEOUT_PRODUCER);
    }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");

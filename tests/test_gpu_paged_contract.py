@@ -146,3 +146,40 @@ def test_error_of_long_sequences_is_within_the_weights_rounding():
             o, _ = _ops().paged_gqa_fwd(q.cuda(), k.cuda(), v.cuda(), table.cuda(), _i32(lens).cuda(), cu_q=_i32(cu).cuda(),
                                         shared_prefix=prefix, max_new=max(new))
         assert within_weights(o, o64, q, k, v, table, lens, cu, prefix, True)
+
+
+SHORTER = [  # new, lens, Hq, Hkv, D, page, shared prefix: nobody is as long as the prefix
+    ([1, 1, 2], [50, 20, 7], 4, 2, 64, 16, 96),
+    ([1] * 24, [100 + 13 * i for i in range(24)], 8, 2, 128, 32, 900),
+    ([40, 3], [300, 170], 8, 2, 64, 64, 640),
+    ([1, 5], [0, 3], 4, 4, 128, 8, 128),
+    ([60, 0, 60], [130, 0, 129], 4, 2, 128, 16, 2048),
+    ([300], [310], 4, 2, 64, 16, 1024),
+    ([2] * 9, [33] * 9, 3, 3, 64, 24, 480),                 # pages that are not for the tiles
+    ([1, 0, 1], [40, 0, 60], 4, 2, 64, 16, 256),            # the slot without a token claims a length, see below
+]
+
+
+@pytest.mark.parametrize("case", SHORTER, ids=lambda c: f"{sum(c[0])}tok{len(c[0])}seq{c[4]}p{c[5]}s{c[6]}")
+@pytest.mark.parametrize("tag", ["bf16", "f16"])
+@pytest.mark.parametrize("causal", [True, False])
+def test_sequences_shorter_than_the_shared_prefix(case, tag, causal, prefix_units):
+    """What lies behind every sequence's end may hold anything, also where a prefix is said to be: it is NaN here."""
+    new, lens, Hq, Hkv, D, page, prefix = case
+    dt = {"bf16": torch.bfloat16, "f16": torch.float16}[tag]
+    ops = _ops()
+    k, v, table = make_cache([max(n, prefix) for n in lens], Hkv, D, page, dt, "hnd", 21, prefix)
+    last = max(lens)                                       # positions [0, last) of the shared pages have been written
+    for p in range(last, prefix // page * page):
+        k[table[0, p // page], :, p % page] = v[table[0, p // page], :, p % page] = float("nan")
+    cu = [0]
+    for n in new:
+        cu.append(cu[-1] + n)
+    q = (torch.randn(cu[-1] + 2, Hq, D, generator=torch.Generator().manual_seed(5)) * 1.5).to(dt)
+    told = [n if m else 250 for n, m in zip(lens, new)] if 0 in new and last == 60 else lens
+    o, lse = ops.paged_gqa_fwd(q.cuda(), k.cuda(), v.cuda(), table.cuda(), _i32(told).cuda(), cu_q=_i32(cu).cuda(), shared_prefix=prefix, causal=causal)
+    o64, lse64 = oracle.paged_attention(q, k, v, table, lens, cu, prefix, causal)
+    assert within_weights(o, o64, q, k, v, table, lens, cu, prefix, causal)
+    seen = torch.isfinite(lse64)
+    assert torch.equal(torch.isfinite(lse.cpu()), seen) and (o.cpu()[~seen] == 0).all()
+    assert ((lse.cpu().double() - lse64)[seen].abs() <= 2.0 ** -16 + 2.0 ** -23 * lse64[seen].abs()).all() and ops.kernel_status() == 0
