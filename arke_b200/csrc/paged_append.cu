@@ -185,7 +185,10 @@ __global__ void __launch_bounds__(128) paged_append_vec_kernel(const AppendParam
   }
 }
 
-// any even head dimension, any alignment: one element pair per thread
+// Any even head dimension, any alignment: one element pair per thread, two bytes at a time.  6000 tokens of 32 / 8 heads
+// of 120, or of 128 at an odd offset: 161 and 169 us, 0.87 TB/s, against 28.7 us of the kernel above; 256 tokens 9.6
+// against 4.1 us.  Bound by the loads' number.  No path of this library makes such rows (its projections are contiguous
+// with heads of 64 and 128); who has long ones copies them to an aligned buffer first.
 template <typename T, typename TT>
 __global__ void __launch_bounds__(128) paged_append_scalar_kernel(const AppendParams p) {
   const int t = blockIdx.x / p.blocks_per_token;

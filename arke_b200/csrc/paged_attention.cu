@@ -24,10 +24,10 @@
 //
 // Bound: HBM.  Few rows make 2 * R flops per byte, far below the ridge, so tcgen05 with its 128-row
 // tiles could only add latency here.  64 ragged sequences of up to 8192 positions (32 / 8 heads, D = 128,
-// 1.25 GB): 197 us, 6.35 TB/s, 98 % of the measured copy rate; with the four warps of a CTA on one tile, a
+// 1.25 GB): 200 us, 6.25 TB/s, 97 % of the measured copy rate; with the four warps of a CTA on one tile, a
 // barrier per unit and a drained ring between units it was 222 us, and 256 short sequences (5 tiles of
 // 64 keys) lost almost half their time.  Short calls are a chain of latencies (lengths, table, keys,
-// partials, join: one sequence of 1000 positions 13.4 us in a graph, 4.1 MB).
+// partials, join: one sequence of 1000 positions 14 us in a graph, 4.1 MB).
 #include "paged_att.cuh"
 #include <limits.h>
 #include <math.h>

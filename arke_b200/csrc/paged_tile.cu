@@ -18,7 +18,7 @@
 // Bound: the softmax arithmetic per SM (about 2900 cycles per 128-key step of two tiles, against 2048 of tensor
 // core work), as in gqa_fwd_kernel; a step streams 64 KB, at that pace 22 B per clock and SM, just the HBM rate.
 // Measured 1.7 us a step (tensor pipe 56 % active) and about 10 us a CTA for its start and end.  Two chunks of 512
-// tokens over 8192 positions (32 / 8 heads, D = 128, 133 GFLOP): 134 us, 0.99 PFLOP/s on 128 of 148 SMs.  A shared
+// tokens over 8192 positions (32 / 8 heads, D = 128, 133 GFLOP): 135 us, 0.99 PFLOP/s on 128 of 148 SMs.  A shared
 // prefix beside streamed keys of the sequences' own: see plan_paged_tiles.
 #include "paged_att.cuh"
 #include <math.h>

@@ -22,14 +22,18 @@
 // A thread-block cluster owns a row: each CTA stages its slice of the row in shared memory (read once
 // from HBM) and the passes run there; histograms, maxima and sums meet through distributed shared memory.
 //
-// Bound: instructions.  A pass costs a logit 10 to 60 of them against the 4 bytes that HBM delivers it in, and two CTAs
-// of 512 threads issue two a cycle (phases wait for one another).  One row of 32000 f32 with top-p: 16 us, seven
-// cluster barriers and as many passes of latency.  64 rows of 128256 bf16 with mixed filters: 53 us; all with top-p
-// 67 us, of which 16 us are the weighted histogram (three shared atomics a logit at 16 cycles a warp each: bank
-// conflicts, not the form of the atomic).  256 rows of 128256 f32 unfiltered: 111 us where the settings are arrays, and
-// so unknown to the host, else 96 us; 18 % of these flat rows are decided by exact sums after all.  Measured and not
-// kept: 256 threads or no staging (unfiltered 92 us, but top-p 80 to 145 us), 1024 threads (257 us), the estimate while
-// the row streams in (one barrier less, but registers spill).
+// Bound: phases.  A row is a chain of passes with barriers of the CTA and the cluster between them, and two CTAs of 512
+// threads per SM (three without bins) do not cover one another's waits: warps spend a third of their time at barriers,
+// 42 to 53 % of the issue slots are taken, HBM runs at 0.4 to 1.4 TB/s.  Behind that come instructions: a pass costs a
+// logit 10 to 60 of them.  One row of 32000 f32 with top-p: 19 us, seven cluster barriers and as many passes of latency.
+// 64 rows of 128256 bf16 with mixed filters: 56 us; all with top-p 68 us, of which some 16 us are the weighted histogram
+// (shared atomics at 16 cycles a warp each: bank conflicts, not the form of the atomic).  256 rows of 128256 f32
+// unfiltered: 114 us where the settings are arrays, and so unknown to the host, else 95 us; 18 % of these flat rows are
+// decided by exact sums after all.  What the exact tails cost: 16.6 / 53 / 62.8 / 112 / 93.5 us without them.
+// Shared memory counts twice: with 6 KB more a CTA still two fit an SM, but the L1 cache gave way and the loads of a row
+// lost 8 % (unfiltered 115 -> 123 us).  Measured and not kept: 256 threads or no staging (unfiltered 92 us, but top-p 80
+// to 145 us), 1024 threads (257 us), the estimate while the row streams in (one barrier less, but registers spill),
+// always the fine histogram (top-p 68 -> 83 us), both histograms as code of their own (registers).
 #include "common.cuh"
 #include "capi_internal.h"
 #include <math.h>
@@ -968,8 +972,7 @@ static int launch_sample_cluster(SampleParams& p, cudaStream_t st) {
 }
 
 // Without top-k and top-p for any row, the kernel that has neither fits an SM three times instead of twice: 40 registers,
-// no bins.  Worth it from two CTAs an SM on (256 rows of 128256 f32: 117 -> 97 us, with min-p 93 -> 78 us; 512 of 50257 f16:
-// 61 -> 53 us), not below (one row of 32000: 5.3 and 5.4 us) nor where a slice is not staged (16 of 2^20: 37 and 39 us).
+// no bins.  Worth it from two CTAs an SM on (256 rows of 128256 f32: 114 -> 95 us; 512 of 50257 f16: 64 -> 55 us), not below (one row of 32000: 5.3 and 5.4 us) nor where a slice is not staged (16 of 2^20: 37 and 39 us).
 template <typename T, int CS>
 static int launch_sample_filters(SampleParams& p, cudaStream_t st) {
   const bool none = !p.k_row && !p.p_row && p.k == 0 && !(p.p < 1.f);

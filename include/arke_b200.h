@@ -334,6 +334,9 @@ ARKE_B200_API int arke_b200_qkv_rope_paged_append(const void* qkv, int64_t ld, c
  *   A page outside its range: the rows that see one of its positions are NaN, o and lse, and other rows of that
  *   sequence may be (of the batch, when it lies in the shared prefix).  A length outside its range: every row of
  *   that sequence is NaN.  Both set status code 8.
+ *   Accuracy: scores, sums and partial results are fp32.  The weights meet the values with 17 bits or more; where many
+ *   rows read the same keys (more than 32 rows times heads per key head of a sequence, or a prefix computed apart) they
+ *   are rounded to the cache's type first, which moves a result by half a step of sum_j p_j |v_j| at most.
  *   workspace: arke_b200_paged_gqa_workspace(...) bytes, 256-byte aligned; contents need no
  *   initialisation and nothing is kept in it between calls; calls that may overlap need one each. */
 ARKE_B200_API size_t arke_b200_paged_gqa_workspace(int64_t T, int64_t batch, int64_t Hq, int64_t Hkv, int64_t D,
@@ -351,7 +354,8 @@ ARKE_B200_API int arke_b200_paged_gqa_fwd(const void* q, int64_t q_stride_token,
  *          all; the first is always kept);
  *   min_p  keeps w_i >= min_p (0: all);
  *   token  = the first kept index i, in vocabulary order, with sum_{j <= i, kept} w_j > u * Z, Z the sum
- *            of what is kept;  logprob [B] (may be NULL) = log(w_token / Z).
+ *            of what is kept;  logprob [B] (may be NULL) = log(w_token / Z), rounded once; in rows that
+ *            neither top_k nor top_p cuts, Z may be a sum of single-precision weights, and logprob off by up to 2^-17.
  * temperature <= 0: the arg max (lowest index), logprob 0.  A NaN logit counts as -inf, which is never
  * chosen; a row of -inf alone gives token -1, logprob -inf.  u outside [0, 1) is clamped; at u = 0 the first
  * kept token whose weight is not zero in 64 bits is chosen.  Decisions are those of 64-bit arithmetic and do not
