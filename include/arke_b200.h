@@ -326,7 +326,8 @@ ARKE_B200_API int arke_b200_qkv_rope_paged_append(const void* qkv, int64_t ld, c
  *   q and the cache; lse [T, Hq] fp32 natural-log logsumexp (may be NULL).  A row that sees nothing:
  *   o = 0, lse = -inf.  softmax_scale <= 0 selects 1/sqrt(D).  A key that a row does not see may hold
  *   anything; so may memory behind a sequence's end.  A NaN or infinity among the values of a sequence's
- *   own positions can reach rows that do not see that position (a weight of 0 times it is NaN).
+ *   own positions can reach its rows that do not see that position (a weight of 0 times it is NaN), in a shared
+ *   prefix rows of every sequence.
  *   shared_prefix: the first positions [0, shared_prefix) of every sequence are the same (of a shorter one,
  *   all that it has; behind the longest sequence nothing is read).  Their whole
  *   pages are read through sequence 0's row of the block table, and once for the whole batch where that
